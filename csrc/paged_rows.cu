@@ -12,13 +12,16 @@
 // e4m3 pools: an e4m3 value is exact in f16, so the products run in f16 on the stored bytes, unscaled. The row of Q is
 // brought to [2^14, 2^15) by a power of two first (exact but for values 2^-29 below the row's largest). The key's
 // scale multiplies the fp32 score; the value's, 2^e, enters the exponent: w = 2^(s + e - M), o = sum w v8, l = sum w
-// 2^-e, with M the running maximum of s + e. P is rounded to f16 (bf16 pools: bf16, the type of V) for its product;
-// the row sum keeps the unrounded fp32 values.
+// 2^-e, with M the running maximum of s + e, less 15: weights reach 2^15. P is rounded to f16 (bf16 pools: bf16, the
+// type of V) for its product; the row sum keeps the unrounded fp32 values. One token can lie far above the others in s +
+// e and still add nothing to a column (a zero value, whose scale is 1, or a single loud channel), so weights of any size
+// must keep their bits: where a tile has weights below 2^-16 (the least that f16 rounds as finely as bf16), what the
+// rounding left of them is multiplied again, 2^40 up, into accumulators that are scaled along.
 //
-// One step of 64 sequences of up to 16384 tokens, 8 key heads of 128, e4m3 (1.34 GB): 270 us and 9 us for the merge,
-// 5.0 TB/s of the copy's 6.6; the ALU pipe is 60 % busy, so the conversions and the softmax of padded rows bound it
-// now, not the loads (three CTAs a SM with two stages: the same time). 8 captions of 320 tokens: 8 us a call, all
-// latency.
+// One step of 64 sequences of up to 16384 tokens, 8 key heads of 128, e4m3 (1.34 GB): 303 us a call, 9 of them the
+// merge, 4.4 TB/s of the copy's 6.6 (293 without the look for small weights; the ALU pipe is 60 % busy, so the
+// conversions and the softmax of padded rows bound it, not the loads; three CTAs a SM with two stages: the same time).
+// 8 captions of 320 tokens: 8 us a call, all latency.
 #include <ATen/cuda/CUDAContext.h>
 #include <torch/extension.h>
 
@@ -36,6 +39,11 @@ using bf16 = __nv_bfloat16;
 namespace {
 
 constexpr int kWarps = 4, kStages = 3, kRows = 16;
+// e4m3 pools: the largest weight, 2^kTop; the least that f16 rounds to 2^-9 of it; and what the remainders of smaller
+// ones, at most 2^-25, are lifted by, at most twice (to 2^-96 of weights up to 2^15; the accumulators then stay below
+// 512 keys * 448 * 2^15 * 2^80 < 2^113)
+constexpr float kTop = 15.f, kLeastWeight = 0x1p-16f, kLift = 0x1p40f;
+constexpr int kLifts = 2;
 constexpr int kStageBytes = 8192;  // K and V of one warp's tile
 
 template <int D, bool Q8>
@@ -97,6 +105,26 @@ __device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
   __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<uint32_t*>(&h);
 }
+__device__ __forceinline__ __half2 as_half2(uint32_t w) { return *reinterpret_cast<__half2*>(&w); }
+
+// e4m3 pools: O += P V for the 16 keys of step kt of the tile's values at shared-memory address v
+template <int D>
+__device__ __forceinline__ void add_pv8(float (&o)[D / 8][4], const uint32_t (&p)[4], uint32_t v, int kt, int lane) {
+  // matrices: keys 0-7 | 8-15 | 0-7 | 8-15 with columns 0-15 | 0-15 | 16-31 | 16-31; a register holds two columns of
+  // two keys, sorted by column before the conversion
+#pragma unroll
+  for (int d = 0; d < D / 32; ++d) {
+    uint32_t r[4];
+    ldsm4t(r, v + Tile<D, true>::off(kt * 16 + (lane & 15), d * 2 + (lane >> 4)));
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint32_t u0 = __byte_perm(r[h * 2], 0, 0x3120), u1 = __byte_perm(r[h * 2 + 1], 0, 0x3120);
+      mma16<true>(o[d * 4 + h * 2], p, e4m3x2_f16x2(u0), e4m3x2_f16x2(u1));
+      mma16<true>(o[d * 4 + h * 2 + 1], p, e4m3x2_f16x2(u0 >> 16), e4m3x2_f16x2(u1 >> 16));
+    }
+  }
+}
+
 __device__ __forceinline__ float quad_max(float v) {
   v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
   return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
@@ -306,7 +334,8 @@ __global__ void __launch_bounds__(kWarps * 32, 2) paged_rows_kernel(const PagedA
     float ms[2];
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
-      const float mn = fmaxf(m[r], quad_max(mt[r]));
+      const float mq = quad_max(mt[r]), top = Q8 && mq - (mq - kTop) <= kTop ? mq - kTop : mq;  // (rounding, infinities)
+      const float mn = fmaxf(m[r], top);
       ms[r] = mn == -INFINITY ? 0.f : mn;  // no visible key yet: weights 2^(-inf) = 0
       const float c = ex2_ftz(m[r] - ms[r]);
       m[r] = mn;
@@ -318,9 +347,10 @@ __global__ void __launch_bounds__(kWarps * 32, 2) paged_rows_kernel(const PagedA
       }
     }
     // ---- P and O += P V
+    const uint32_t vst = st + kStageBytes / 2;
+    uint32_t pf[KT / 16][4];
 #pragma unroll
     for (int kt = 0; kt < KT / 16; ++kt) {
-      uint32_t pf[4];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         float(&x)[4] = s[kt * 2 + h];
@@ -329,33 +359,64 @@ __global__ void __launch_bounds__(kWarps * 32, 2) paged_rows_kernel(const PagedA
           x[c] = ex2_ftz(x[c] - ms[c >> 1]);
           l[c >> 1] += Q8 ? x[c] * un[kt * 2 + h][c & 1] : x[c];
         }
-        pf[h * 2] = Q8 ? pack_half(x[0], x[1]) : pack_bf16(x[0], x[1]);
-        pf[h * 2 + 1] = Q8 ? pack_half(x[2], x[3]) : pack_bf16(x[2], x[3]);
+        pf[kt][h * 2] = Q8 ? pack_half(x[0], x[1]) : pack_bf16(x[0], x[1]);
+        pf[kt][h * 2 + 1] = Q8 ? pack_half(x[2], x[3]) : pack_bf16(x[2], x[3]);
       }
-      const uint32_t vst = st + kStageBytes / 2;
       if (Q8) {
-        // matrices: keys 0-7 | 8-15 | 0-7 | 8-15 with columns 0-15 | 0-15 | 16-31 | 16-31; a register holds two
-        // columns of two keys, sorted by column before the conversion
-#pragma unroll
-        for (int d = 0; d < D / 32; ++d) {
-          uint32_t r[4];
-          ldsm4t(r, vst + T::off(kt * 16 + (lane & 15), d * 2 + (lane >> 4)));
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const uint32_t u0 = __byte_perm(r[h * 2], 0, 0x3120), u1 = __byte_perm(r[h * 2 + 1], 0, 0x3120);
-            mma16<true>(o[d * 4 + h * 2], pf, e4m3x2_f16x2(u0), e4m3x2_f16x2(u1));
-            mma16<true>(o[d * 4 + h * 2 + 1], pf, e4m3x2_f16x2(u0 >> 16), e4m3x2_f16x2(u1 >> 16));
-          }
-        }
+        add_pv8<D>(o, pf[kt], vst, kt, lane);
       } else {
         // matrices: keys 0-7 | 8-15 | 0-7 | 8-15 with columns 0-7 | 0-7 | 8-15 | 8-15
 #pragma unroll
         for (int d = 0; d < D / 16; ++d) {
           uint32_t r[4];
           ldsm4t(r, vst + T::off(kt * 16 + (lane & 15), d * 2 + (lane >> 4)));
-          mma16<false>(o[d * 2], pf, r[0], r[1]);
-          mma16<false>(o[d * 2 + 1], pf, r[2], r[3]);
+          mma16<false>(o[d * 2], pf[kt], r[0], r[1]);
+          mma16<false>(o[d * 2 + 1], pf[kt], r[2], r[3]);
         }
+      }
+    }
+    if (Q8) {  // weights that f16 cut short (masked keys, weight 0, look like them at first)
+      bool low = false;
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        __half2 least = as_half2(pf[0][r]);
+#pragma unroll
+        for (int i = 1; i < KT / 8; ++i) least = __hmin2(least, as_half2(pf[i >> 1][(i & 1) * 2 + r]));
+        low |= last[r] >= 0 && !__hbge2(least, __float2half2_rn(kLeastWeight));
+      }
+      float lifted = 1.f;
+      if (__any_sync(0xffffffffu, low)) {
+#pragma unroll 1
+        for (int i = 0; i < kLifts; ++i) {
+          bool rest = false;
+#pragma unroll
+          for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {  // the remainder, exact
+              float& x = s[j][c];
+              x = fabsf(x) < kLeastWeight ? x - __half2float(__float2half_rn(x)) : 0.f;
+              rest |= x != 0.f;
+              x *= kLift;
+            }
+          if (!__any_sync(0xffffffffu, rest)) break;
+          lifted *= kLift;
+#pragma unroll
+          for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) o[d][c] *= kLift;
+#pragma unroll
+          for (int kt = 0; kt < KT / 16; ++kt) {
+            const float(&x)[4] = s[kt * 2], (&y)[4] = s[kt * 2 + 1];
+            const uint32_t pr[4] = {pack_half(x[0], x[1]), pack_half(x[2], x[3]), pack_half(y[0], y[1]),
+                                    pack_half(y[2], y[3])};
+            add_pv8<D>(o, pr, vst, kt, lane);
+          }
+        }
+        const float down = 1.f / lifted;
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) o[d][c] *= down;
       }
     }
   }
