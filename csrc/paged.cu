@@ -203,19 +203,17 @@ __global__ void __launch_bounds__(256) paged_merge_kernel(const PagedAttnArgs a)
   float l = 0.f, acc[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) acc[e] = 0.f;
-  if (m != -INFINITY) {
 #pragma unroll 4
-    for (int i = 0; i < used; ++i) {
-      const float2 x = ml[i * units + at];
-      if (x.x == -INFINITY) continue;  // a split without a visible key
-      const float w = ex2_ftz(x.x - m);
-      l += x.y * w;
-      const float* src = a.part + (i * units + at) * D + lane * E;
+  for (int i = 0; i < used; ++i) {
+    const float2 x = ml[i * units + at];
+    if (paged_saw_nothing(x.x, x.y)) continue;
+    const float w = ex2_ftz(x.x - m);
+    l += x.y * w;
+    const float* src = a.part + (i * units + at) * D + lane * E;
 #pragma unroll
-      for (int e = 0; e < E; ++e) acc[e] += src[e] * w;
-    }
+    for (int e = 0; e < E; ++e) acc[e] += src[e] * w;
   }
-  const float inv = l > 0.f ? 1.f / l : 0.f;
+  const float inv = paged_inv(l);
 #pragma unroll
   for (int e = 0; e < E; e += 2)
     *reinterpret_cast<uint32_t*>(a.o + at * D + lane * E + e) = pack_bf16(acc[e] * inv, acc[e + 1] * inv);

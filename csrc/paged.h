@@ -83,9 +83,15 @@ __device__ __forceinline__ int paged_used_splits(const PagedAttnArgs& a, int tot
   return max(1, (total + a.split_len - 1) / a.split_len);
 }
 
-// log-sum-exp (natural) of a row from its maximum (log2 units) and its sum relative to it
+// A row, or a part of it, that saw no key has m = -inf and l = 0. A NaN score moves no maximum (fmaxf drops it) but makes
+// the sum NaN, so m alone does not tell: the sum decides, here and in every merge.
+__device__ __forceinline__ bool paged_saw_nothing(float m, float l) { return m == -INFINITY && l == 0.f; }
+
+// log-sum-exp (natural) of a row from its maximum (log2 units) and its sum relative to it; NaN where the sum is
 __device__ __forceinline__ float paged_lse(float m, float l) {
-  return l > 0.f ? (m + log2f(l)) * 0.69314718055994531f : -INFINITY;
+  return l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
 }
+// what the unnormalised output is multiplied by
+__device__ __forceinline__ float paged_inv(float l) { return l == 0.f ? 0.f : 1.f / l; }
 
 }  // namespace ng

@@ -464,12 +464,12 @@ __global__ void __launch_bounds__(kWarps * 32, 2) paged_rows_kernel(const PagedA
     for (int w = 0; w < kWarps; ++w) {
       const float4 x = *reinterpret_cast<const float4*>(so + (w * kRows + r) * LD + c);
       v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
-      if (mc != -INFINITY) lc += s_l[w][r] * ex2_ftz(s_m[w][r] - mc);
+      lc += mc == -INFINITY ? s_l[w][r] : s_l[w][r] * ex2_ftz(s_m[w][r] - mc);
     }
     const int tok = (rt * kRows + r) / G;
     const int64_t at = (int64_t)(row0 + tok) * a.H + hk * G + rt * kRows + r - tok * G;  // (packed row, head)
     if (one) {
-      const float inv = lc > 0.f ? 1.f / lc : 0.f;
+      const float inv = paged_inv(lc);
       *reinterpret_cast<uint2*>(a.o + at * D + c) =
           make_uint2(pack_bf16(v.x * inv, v.y * inv), pack_bf16(v.z * inv, v.w * inv));
       if (c == 0) a.lse[at] = paged_lse(mc, lc);

@@ -788,7 +788,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc_fence_after();
       }
       const int64_t at = (int64_t)(s.row0 + tok) * a.H + s.hk * G + r - tok * G;  // (packed row, head)
-      const float inv = l > 0.f ? 1.f / l : 0.f;
+      const float inv = paged_inv(l);
       const int slot = 2 * blockIdx.x + (s.j0 > 0 ? 0 : 1);
       const int64_t prow = (int64_t)slot * 2 * kTileRows + X * kTileRows + row;
 #pragma unroll 1
@@ -860,17 +860,17 @@ __global__ void __launch_bounds__(256) paged_tiles_merge_kernel(const __grid_con
     float l = 0.f, acc[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) acc[e] = 0.f;
-    for (int k = c - 1; k <= last && m != -INFINITY; ++k) {
+    for (int k = c - 1; k <= last; ++k) {
       if (k >= c && t.cuts[k * 8] >= t.cuts[k * 8 + 6]) continue;
       const int64_t at = (int64_t)(k < c ? 2 * k + 1 : 2 * k) * 2 * kTileRows + row;
       const float2 x = ml[at];
-      if (x.x == -INFINITY) continue;
+      if (paged_saw_nothing(x.x, x.y)) continue;
       const float f = ex2_ftz(x.x - m);
       l += x.y * f;
 #pragma unroll
       for (int e = 0; e < E; ++e) acc[e] += t.part[at * D + lane * E + e] * f;
     }
-    const float inv = l > 0.f ? 1.f / l : 0.f;
+    const float inv = paged_inv(l);
     const int r = r0 + row, tok = r / G;
     const int64_t at = (int64_t)(row0 + tok) * a.H + hk * G + r - tok * G;
 #pragma unroll

@@ -3,7 +3,7 @@ the inputs and the tolerances are those of test_paged_gpu.py."""
 import pytest
 import torch
 
-from test_paged_gpu import _check, _setup
+from test_paged_gpu import _attn_ref, _check, _q, _setup
 
 pytestmark = pytest.mark.gpu
 
@@ -49,3 +49,34 @@ def test_one_loud_channel_of_high_weight(kind, n, t, D):
         for loud in (2.0 ** 8, 2.0 ** 20, 2.0 ** 40):
             q, kv, table, cu = _one_loud(n, t, D, kind, size, 12, loud, 0.0, seed=n + D)
             _check(q, kv, table, cu, [n], [t])
+
+
+# ------------------------------------------------------------------------------------------------------ NaN stays NaN
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+@pytest.mark.parametrize("n", [1, 8, 200])
+@pytest.mark.parametrize("t", [300, 4097, 16385])  # one split; the last key of the longer ones is alone in its split
+@pytest.mark.parametrize("where", ["query", "first key", "last key"])
+def test_nan_is_not_an_empty_row(kind, n, t, where):
+    """A NaN query, or a NaN key that a row sees, makes that row's output and log-sum-exp NaN, split or not; a row that
+    saw nothing (o = 0, lse = -inf) is something else, and rows that do not see the NaN keep their results."""
+    from nano_gpic_b200.ops import paged as P
+    D, H, Hk = 128, 4, 2
+    kv, table, cu, _, tot = _setup([n], [t], Hk, D, 16, kind)
+    g = torch.Generator(device="cuda").manual_seed(t + n)
+    k, v = (torch.randn(t, Hk * D, device="cuda", generator=g).bfloat16() for _ in range(2))
+    q = _q(n, H, D)
+    if where == "query":
+        q[n // 2, D + 3] = float("nan")  # of head 1
+    else:
+        k[0 if where == "first key" else t - 1, 7] = float("nan")  # of key head 0: heads 0 and 1
+    P.cache_write(kv, k, v, table, torch.zeros(1, dtype=torch.int32, device="cuda"),
+                  torch.tensor([0, t], dtype=torch.int32, device="cuda"))
+    o, lse = P.paged_attn(q, kv, table, tot, cu, n, t)
+    ro, rl, A, se = _attn_ref(q, kv, table, [n], [t], D ** -0.5)
+    bad = rl.isnan()
+    assert int(bad.sum()) == {"query": 1, "first key": 2 * n, "last key": 2}[where]
+    o = o.double().view(n, H, D)
+    assert torch.equal(lse.isnan(), bad) and torch.equal(o.isnan(), bad[..., None].expand_as(o))
+    err, tol = (o - ro).abs(), A * (2 ** -7 + 2 ** -12 + 3 * se[..., None])
+    assert (err <= tol)[~bad].all()
+    assert ((lse.double() - rl)[~bad].abs() <= (se + 2 ** -19 * (1 + rl.abs()))[~bad]).all()
