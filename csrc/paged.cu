@@ -409,7 +409,11 @@ std::vector<at::Tensor> paged_attn(const at::Tensor& q, const at::Tensor& pk, co
   a.T = (int)T;
   a.H = (int)H;
   a.max_new = (int)max_new;
-  a.max_total = (int)max_total;
+  a.bound_total = (int)max_total;
+  // a bound is often loose (a captured graph's, "any length"): splits and their workspace go by what the table holds
+  const int64_t held = std::min<int64_t>(max_total, (int64_t)a.p.width << a.p.page_shift);
+  TORCH_CHECK(held <= kMaxTokens, "paged: max_total and the table allow a sequence of too many tokens");
+  a.max_total = (int)held;
   a.causal = causal;
   a.scale_log2 = (float)(scale * 1.4426950408889634);
   a.err = status_word();

@@ -64,7 +64,9 @@ struct PagedAttnArgs {
   float* lse;        // [T, H]
   const int* total;
   const int* cu;
-  int B, T, H, max_new, max_total, causal;
+  int B, T, H, causal;
+  int max_new, max_total;  // what the launch is sized for: no more than the table can hold
+  int bound_total;         // the caller's bound
   float scale_log2;  // softmax scale * log2(e)
   int* err;
   // work split over the keys: split i of a sequence takes keys [i split_len, (i + 1) split_len)
@@ -73,6 +75,17 @@ struct PagedAttnArgs {
 };
 
 constexpr int kSMs = 148;
+constexpr int kMaxTokens = INT32_MAX - 8192;  // of a sequence: positions a tile past the end stay inside an int
+
+// Tokens of a sequence with n new rows, its entry in `total` given, that the kernels work on. The status word is set
+// where it is beyond the caller's bound, or beyond what its row of the table holds.
+__device__ __forceinline__ int paged_total(const PagedAttnArgs& a, int n, int total) {
+  if (total > a.bound_total)
+    raise_error(a.err, kErrBound);
+  else if (n > 0 && total > a.max_total)
+    raise_error(a.err, kErrPage);
+  return max(0, min(total, a.max_total));
+}
 
 void paged_rows_launch(PagedAttnArgs a, cudaStream_t st);
 void paged_tiles_launch(PagedAttnArgs a, cudaStream_t st);

@@ -154,9 +154,8 @@ __global__ void __launch_bounds__(kWarps * 32, 2) paged_rows_kernel(const PagedA
   const int G = a.H / a.p.Hk;
   const int row0 = max(0, __ldg(a.cu + b));
   const int n = max(0, min(__ldg(a.cu + b + 1), a.T) - row0);
-  int total = __ldg(a.total + b);
-  if ((n > a.max_new || total > a.max_total) && threadIdx.x == 0) raise_error(a.err, kErrBound);
-  total = max(0, min(total, a.max_total));
+  if (n > a.max_new && threadIdx.x == 0) raise_error(a.err, kErrBound);
+  const int total = paged_total(a, n, __ldg(a.total + b));
   const int R = min(kRows, n * G - rt * kRows);  // rows of this tile; row r: token (rt * 16 + r) / G, head hk G + rest
   if (R <= 0) return;
   const int used = paged_used_splits(a, total);

@@ -3,7 +3,7 @@ the inputs and the tolerances are those of test_paged_gpu.py."""
 import pytest
 import torch
 
-from test_paged_gpu import _attn_ref, _check, _q, _setup
+from test_paged_gpu import _attn_ref, _check, _fill, _q, _setup
 
 pytestmark = pytest.mark.gpu
 
@@ -80,3 +80,28 @@ def test_nan_is_not_an_empty_row(kind, n, t, where):
     err, tol = (o - ro).abs(), A * (2 ** -7 + 2 ** -12 + 3 * se[..., None])
     assert (err <= tol)[~bad].all()
     assert ((lse.double() - rl)[~bad].abs() <= (se + 2 ** -19 * (1 + rl.abs()))[~bad]).all()
+
+
+# -------------------------------------------------------------------------------------------------------- loose bounds
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+@pytest.mark.parametrize("n", [1, 150])
+@pytest.mark.parametrize("bound", [1 << 30, (1 << 31) - 1])
+def test_any_length_as_bound(kind, n, bound):
+    """max_total far above what the table can hold ("any length"): the same results, from a workspace that goes by the
+    table; a sequence that the table cannot hold still sets the status word."""
+    from nano_gpic_b200.ops import paged as P
+    from nano_gpic_b200.ops import status
+    new, total = [n, n, n], [5000, 2100, 170]
+    kv, table, cu, _, _ = _setup(new, total, 2, 128, 16, kind)
+    _fill(kv, table, total)
+    q = _q(3 * n, 16, 128)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    P.paged_attn(q, kv, table, torch.tensor(total, dtype=torch.int32, device="cuda"), cu, n, bound)
+    assert torch.cuda.max_memory_allocated() - before < 1 << 28
+    _check(q, kv, table, cu, new, total, bound=(n, bound))
+    long = torch.tensor([5000, table.shape[1] * 16 + 1, 170], dtype=torch.int32, device="cuda")
+    P.paged_attn(q, kv, table, long, cu, n, bound)
+    with pytest.raises(RuntimeError, match="page table"):
+        status.check()
