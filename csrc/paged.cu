@@ -396,7 +396,7 @@ std::vector<at::Tensor> paged_attn(const at::Tensor& q, const at::Tensor& pk, co
   TORCH_CHECK(max_new >= 0 && max_total >= 0 && max_new <= INT32_MAX && max_total <= INT32_MAX,
               "paged: max_new / max_total out of range");
   const int64_t H = q.size(1) / D;
-  TORCH_CHECK(T * H <= INT32_MAX, "paged: too many rows");
+  TORCH_CHECK(T * H <= INT32_MAX - 256, "paged: too many rows");
   at::Tensor o = at::empty({T, H * D}, q.options()), lse = at::empty({T, H}, q.options().dtype(at::kFloat));
   if (T == 0) return {o, lse};
   a.q = reinterpret_cast<const bf16*>(q.data_ptr());
@@ -408,6 +408,8 @@ std::vector<at::Tensor> paged_attn(const at::Tensor& q, const at::Tensor& pk, co
   a.B = (int)B;
   a.T = (int)T;
   a.H = (int)H;
+  a.bound_new = (int)max_new;
+  max_new = std::min(max_new, T);  // row tiles, their first rows in 32 bits, are counted for rows that exist
   a.max_new = (int)max_new;
   a.bound_total = (int)max_total;
   // a bound is often loose (a captured graph's, "any length"): splits and their workspace go by what the table holds

@@ -65,8 +65,8 @@ struct PagedAttnArgs {
   const int* total;
   const int* cu;
   int B, T, H, causal;
-  int max_new, max_total;  // what the launch is sized for: no more than the table can hold
-  int bound_total;         // the caller's bound
+  int max_new, max_total;  // what the launch is sized for: no more than q's rows, no more than the table can hold
+  int bound_new, bound_total;  // the caller's bounds
   float scale_log2;  // softmax scale * log2(e)
   int* err;
   // work split over the keys: split i of a sequence takes keys [i split_len, (i + 1) split_len)

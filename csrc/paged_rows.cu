@@ -154,7 +154,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) paged_rows_kernel(const PagedA
   const int G = a.H / a.p.Hk;
   const int row0 = max(0, __ldg(a.cu + b));
   const int n = max(0, min(__ldg(a.cu + b + 1), a.T) - row0);
-  if (n > a.max_new && threadIdx.x == 0) raise_error(a.err, kErrBound);
+  if (n > a.bound_new && threadIdx.x == 0) raise_error(a.err, kErrBound);
   const int total = paged_total(a, n, __ldg(a.total + b));
   const int R = min(kRows, n * G - rt * kRows);  // rows of this tile; row r: token (rt * 16 + r) / G, head hk G + rest
   if (R <= 0) return;

@@ -105,3 +105,18 @@ def test_any_length_as_bound(kind, n, bound):
     P.paged_attn(q, kv, table, long, cu, n, bound)
     with pytest.raises(RuntimeError, match="page table"):
         status.check()
+
+
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+@pytest.mark.parametrize("n", [1, 150])
+@pytest.mark.parametrize("bound", [1 << 20, 1 << 29, (1 << 31) - 1])
+def test_any_number_of_new_rows_as_bound(kind, n, bound):
+    """max_new far above the rows of q: the launch goes by q (eight query heads a key head: rows times heads of such a
+    bound pass 2^31), results as with the tight bound of the same kernel."""
+    new, total = [n], [400]
+    kv, table, cu, _, _ = _setup(new, total, 1, 64, 16, kind)
+    _fill(kv, table, total)
+    q = _q(n, 8, 64)
+    a = _check(q, kv, table, cu, new, total, bound=(n, 400))
+    b = _check(q, kv, table, cu, new, total, bound=(bound, 400))
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
