@@ -399,6 +399,11 @@ std::vector<at::Tensor> paged_attn(const at::Tensor& q, const at::Tensor& pk, co
   TORCH_CHECK(T * H <= INT32_MAX - 256, "paged: too many rows");
   at::Tensor o = at::empty({T, H * D}, q.options()), lse = at::empty({T, H}, q.options().dtype(at::kFloat));
   if (T == 0) return {o, lse};
+  if (B == 0 || max_new == 0) {  // no row belongs to a sequence, or none may: every row is padding
+    o.zero_();
+    lse.fill_(-INFINITY);
+    if (B == 0) return {o, lse};
+  }
   a.q = reinterpret_cast<const bf16*>(q.data_ptr());
   a.ldq = q.stride(0);
   a.o = reinterpret_cast<bf16*>(o.data_ptr());
@@ -409,7 +414,9 @@ std::vector<at::Tensor> paged_attn(const at::Tensor& q, const at::Tensor& pk, co
   a.T = (int)T;
   a.H = (int)H;
   a.bound_new = (int)max_new;
-  max_new = std::min(max_new, T);  // row tiles, their first rows in 32 bits, are counted for rows that exist
+  // Row tiles, their first rows in 32 bits, are counted for rows that exist; one at least, which sets the status word
+  // where a sequence has rows in spite of max_new = 0.
+  max_new = std::max<int64_t>(1, std::min(max_new, T));
   a.max_new = (int)max_new;
   a.bound_total = (int)max_total;
   // a bound is often loose (a captured graph's, "any length"): splits and their workspace go by what the table holds

@@ -120,3 +120,26 @@ def test_any_number_of_new_rows_as_bound(kind, n, bound):
     a = _check(q, kv, table, cu, new, total, bound=(n, 400))
     b = _check(q, kv, table, cu, new, total, bound=(bound, 400))
     assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+def test_only_padding_rows(kind):
+    """Rows in q that no sequence owns, none at all or max_new = 0: zeros and -inf, as on the CPU, and no error; rows of
+    a sequence in spite of max_new = 0 set the status word."""
+    from nano_gpic_b200.ops import paged as P
+    from nano_gpic_b200.ops import status
+    kv, table, cu, pos, tot = _setup([0, 0], [20, 30], 2, 64, 16, kind)
+    _fill(kv, table, [20, 30])
+    q = _q(5, 4, 64)
+    none = torch.zeros(1, dtype=torch.int32, device="cuda")
+    for call in ((q, kv, table, tot, cu, 0, 30), (q, kv, table[:0], tot[:0], none, 3, 30),
+                 (q, kv, table[:0], tot[:0], none, 0, 0)):
+        o, lse = P.paged_attn(*call)
+        status.check()
+        assert o.shape == (5, 256) and lse.shape == (5, 4) and (o == 0).all() and (lse == float("-inf")).all()
+    P.cache_write(kv, q[:, :128], q[:, :128], table[:0], pos[:0], none)
+    k, _ = P.cache_read(kv, table[:0], pos[:0], none, 5)
+    assert (k == 0).all()
+    P.paged_attn(q, kv, table, tot, torch.tensor([0, 5, 5], dtype=torch.int32, device="cuda"), 0, 30)
+    with pytest.raises(RuntimeError, match="bound"):
+        status.check()
