@@ -246,10 +246,13 @@ PagedPool pool_of(const at::Tensor& k, const at::Tensor& v, const c10::optional<
   TORCH_CHECK(q8 || k.scalar_type() == at::kBFloat16, "paged: the pool must be bf16 or uint8 (e4m3 bytes)");
   TORCH_CHECK(q8 == opt(ksf) && q8 == opt(vsf), "paged: e4m3 pools need both scale pools, bf16 pools none");
   if (q8)
-    for (const at::Tensor& s : {*ksf, *vsf})
+    for (const at::Tensor& s : {*ksf, *vsf}) {
       TORCH_CHECK(s.device() == k.device() && s.scalar_type() == at::kByte && s.is_contiguous() && s.dim() == 3 &&
                       s.size(0) == k.size(0) && s.size(1) == k.size(1) && s.size(2) == k.size(2),
                   "paged: scales must be a contiguous uint8 [pages, heads, page]");
+      TORCH_CHECK(reinterpret_cast<uintptr_t>(s.data_ptr()) % 4 == 0,  // four tokens a copy in csrc/paged_rows.cu
+                  "paged: scale pools must be 4-byte aligned");
+    }
   const int64_t page = k.size(2), D = k.size(3);
   TORCH_CHECK(D == 64 || D == 128, msg("paged: head dim must be 64 or 128, got ", D));
   TORCH_CHECK(page >= 8 && page <= 1024 && (page & (page - 1)) == 0,

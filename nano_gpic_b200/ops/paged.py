@@ -28,7 +28,7 @@ SCALE_LO, SCALE_HI = -62, 63
 
 class PagedKV:
     """Pools k, v [pages, Hk, page, D], bf16 or uint8 (e4m3 bytes, with k_sf, v_sf uint8 [pages, Hk, page] E8M0 scale
-    bytes); D is 64 or 128, page a power of two from 8 to 1024. `PagedKV.empty` allocates one."""
+    bytes, 4-byte aligned); D is 64 or 128, page a power of two from 8 to 1024. `PagedKV.empty` allocates one."""
 
     __slots__ = ("k", "v", "k_sf", "v_sf")
 
@@ -64,6 +64,8 @@ def _check(cache, table, B1, per_seq):
         raise RuntimeError(f"paged: the page size must be a power of two from 8 to 1024, got {page}")
     if (k.dtype == torch.uint8) != (cache.k_sf is not None) or (k.dtype == torch.uint8) != (cache.v_sf is not None):
         raise RuntimeError("paged: e4m3 pools need both scale pools, bf16 pools none")
+    if any(t is not None and t.data_ptr() % 4 for t in (cache.k_sf, cache.v_sf)):
+        raise RuntimeError("paged: scale pools must be 4-byte aligned")
     if table.dim() != 2 or B1.shape[0] != table.shape[0] + 1 or per_seq.shape[0] != table.shape[0]:
         raise RuntimeError("paged: table [B, n], cu [B + 1] and one length or position per sequence expected")
 

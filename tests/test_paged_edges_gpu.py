@@ -143,3 +143,20 @@ def test_only_padding_rows(kind):
     P.paged_attn(q, kv, table, tot, torch.tensor([0, 5, 5], dtype=torch.int32, device="cuda"), 0, 30)
     with pytest.raises(RuntimeError, match="bound"):
         status.check()
+
+
+# ------------------------------------------------------------------------------------------------------------ refusals
+def test_scale_pools_of_odd_alignment_are_refused():
+    """A contiguous scale pool at an odd place of a byte arena: refused on the host by every call."""
+    from nano_gpic_b200.ops import paged as P
+    kv, table, cu, pos, tot = _setup([2, 2], [20, 30], 2, 128, 16, "e4m3")
+    arena = torch.zeros(2 * kv.k_sf.numel() + 8, dtype=torch.uint8, device="cuda")
+    k, q = _q(4, 2, 128), _q(4, 4, 128)
+    for at in (1, 2, 3):
+        odd = arena[at:at + kv.k_sf.numel()].view(kv.k_sf.shape)
+        for sf in ((odd, kv.v_sf), (kv.k_sf, odd)):
+            bad = P.PagedKV(kv.k, kv.v, *sf)
+            for call in (lambda: P.cache_write(bad, k, k, table, pos, cu), lambda: P.cache_read(bad, table, pos, cu, 4),
+                         lambda: P.paged_attn(q, bad, table, tot, cu, 2, 30)):
+                with pytest.raises(RuntimeError, match="paged: scale pools"):
+                    call()
