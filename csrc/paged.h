@@ -4,8 +4,11 @@
 // bytes; e4m3 pools carry one E8M0 scale byte per (token, key head), [pages, Hk, page], value = e4m3 * 2^(byte - 127).
 // Token t of sequence b sits in page table[b, t / page], slot t % page.
 #pragma once
+#include <c10/cuda/CUDAException.h>
 #include <cuda_bf16.h>
 #include <stdint.h>
+
+#include <mutex>
 
 namespace ng {
 
@@ -85,6 +88,22 @@ __device__ __forceinline__ int paged_total(const PagedAttnArgs& a, int n, int to
   else if (n > 0 && total > a.max_total)
     raise_error(a.err, kErrPage);
   return max(0, min(total, a.max_total));
+}
+
+// Allows a kernel `bytes` of dynamic shared memory, once a device: the attribute belongs to the function on the current
+// device. `done` is the kernel's own.
+struct SmemAllowed {
+  std::once_flag device[64];
+};
+template <typename K>
+inline void allow_smem(K* kernel, int bytes, SmemAllowed& done) {
+  int dev = 0;
+  C10_CUDA_CHECK(cudaGetDevice(&dev));
+  auto set = [&] { C10_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes)); };
+  if (dev < 64)
+    std::call_once(done.device[dev], set);
+  else
+    set();
 }
 
 void paged_rows_launch(PagedAttnArgs a, cudaStream_t st);

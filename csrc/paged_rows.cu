@@ -26,7 +26,6 @@
 #include <torch/extension.h>
 
 #include <cuda_fp16.h>
-#include <mutex>
 
 #include "common.cuh"
 #include "paged.h"
@@ -484,10 +483,8 @@ __global__ void __launch_bounds__(kWarps * 32, 2) paged_rows_kernel(const PagedA
 template <int D, bool Q8>
 static void launch_rows(const PagedAttnArgs& a, cudaStream_t st) {
   const int smem = std::max(Tile<D, Q8>::SMEM, kWarps * kRows * (D + 4) * 4);
-  static std::once_flag once;  // the attribute is per function and process
-  std::call_once(once, [&] {
-    C10_CUDA_CHECK(cudaFuncSetAttribute(paged_rows_kernel<D, Q8>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-  });
+  static SmemAllowed allowed;
+  allow_smem(paged_rows_kernel<D, Q8>, smem, allowed);
   const int64_t grid = (int64_t)a.B * a.p.Hk * a.row_tiles * a.splits;
   paged_rows_kernel<D, Q8><<<(int)grid, kWarps * 32, smem, st>>>(a);
   NG_LAUNCH_CHECK();

@@ -34,7 +34,6 @@
 #include <torch/extension.h>
 
 #include <cuda_fp16.h>
-#include <mutex>
 
 #include "common.cuh"
 #include "gemm.h"
@@ -881,11 +880,8 @@ __global__ void __launch_bounds__(256) paged_tiles_merge_kernel(const __grid_con
 
 template <int D, bool Q8>
 static void launch_tiles(const TileArgs& t, int grid, cudaStream_t st) {
-  static std::once_flag once;
-  std::call_once(once, [] {
-    C10_CUDA_CHECK(cudaFuncSetAttribute(paged_tiles_kernel<D, Q8>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                        Lay<D>::SMEM));
-  });
+  static SmemAllowed allowed;
+  allow_smem(paged_tiles_kernel<D, Q8>, Lay<D>::SMEM, allowed);
   const PagedPool& p = t.a.p;
   CUtensorMap mk{}, mv{};
   if (!Q8) {

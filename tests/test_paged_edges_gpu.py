@@ -160,3 +160,19 @@ def test_scale_pools_of_odd_alignment_are_refused():
                          lambda: P.paged_attn(q, bad, table, tot, cu, 2, 30)):
                 with pytest.raises(RuntimeError, match="paged: scale pools"):
                     call()
+
+
+@pytest.mark.skipif(torch.cuda.device_count() < 2, reason="needs a second device")
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+def test_second_device_of_a_process(kind):
+    """Both kernels on one device, then on another of the same process: their shared memory is allowed on each."""
+    from nano_gpic_b200.ops import paged as P
+    for n in (1, 150):
+        new, total = [n, n], [200, 180]
+        kv, table, cu, _, tot = _setup(new, total, 2, 128, 16, kind)
+        _fill(kv, table, total)
+        q = _q(2 * n, 4, 128)
+        want = P.paged_attn(q, kv, table, tot, cu, n, 200)
+        there = [x.to("cuda:1") if x is not None else None for x in (q, table, tot, cu, kv.k, kv.v, kv.k_sf, kv.v_sf)]
+        got = P.paged_attn(there[0], P.PagedKV(*there[4:]), *there[1:4], n, 200)
+        assert all(torch.equal(x, y.to("cuda:0")) for x, y in zip(want, got))
