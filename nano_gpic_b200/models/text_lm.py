@@ -30,12 +30,34 @@ class TextCache:
         self.lens = [0] * seqs  # tokens of each sequence so far
 
 
+WEIGHTS = tuple(f"{n}.weight" for n in (
+    "embed_tokens", "input_layernorm", "post_attention_layernorm", "q_norm", "k_norm", "q_proj", "k_proj", "v_proj",
+    "o_proj", "gate_proj", "up_proj", "down_proj", "norm"))
+# rotary tables that are fixed frequencies and nothing else
+ROPE_TYPES = ("default", "linear", "llama3")
+
+
+def _check_model(model):
+    """Raises for what a Qwen3Model may have and the blocks above do not compute."""
+    c = model.config
+    if set(c.layer_types) != {"full_attention"}:
+        raise ValueError("TextLM: full attention in every layer expected, the model has a sliding window")
+    if c.hidden_act not in ("silu", "swish"):
+        raise ValueError(f"TextLM: hidden_act must be 'silu', got {c.hidden_act!r}")
+    rope = getattr(c, "rope_parameters", None) or getattr(c, "rope_scaling", None) or {}
+    kind = rope.get("rope_type", rope.get("type", "default"))
+    if kind not in ROPE_TYPES or getattr(model.rotary_emb, "attention_scaling", 1.0) != 1.0:
+        raise ValueError(f"TextLM: rotary embedding of type {ROPE_TYPES} without attention scaling expected, got {kind!r}")
+
+
 class TextLM:
-    """Weights of a transformers Qwen3Model, laid out for the kernels."""
+    """Weights of a transformers Qwen3Model, laid out for the kernels. A model with anything these blocks do not compute
+    (biases, a sliding window, another activation, a scaled or length-dependent rotary embedding) is refused."""
 
     def __init__(self, model, fp8=None):
         if fp8 not in (None, "mx"):
             raise ValueError(f"fp8 must be None or 'mx', got {fp8!r}")
+        _check_model(model)
         c = model.config
         self.fp8 = fp8
         self.heads, self.kv_heads = c.num_attention_heads, c.num_key_value_heads
@@ -58,6 +80,9 @@ class TextLM:
             up = torch.cat([sd[p + "mlp.gate_proj.weight"], sd[p + "mlp.up_proj.weight"]]).to(BF16)
             w["qkv"], w["up"] = (MXO.quant(qkv), MXO.quant(up)) if fp8 else (qkv, up)
             self.blocks.append(w)
+        rest = sorted(k for k in sd if not k.startswith("rotary_emb.") and not k.endswith(WEIGHTS))
+        if rest:
+            raise ValueError(f"TextLM: no use for the model's {rest}")
 
     def _norm(self, delta, s, w):
         f = N.add_rms_fwd_mx if self.fp8 else N.add_rms_fwd

@@ -1,0 +1,47 @@
+"""What models/text_lm.py refuses, and how the conditioner keeps it in step with its module."""
+import pytest
+import torch
+
+
+def _qwen3(**kw):
+    transformers = pytest.importorskip("transformers")
+    torch.manual_seed(0)
+    c = dict(vocab_size=97, hidden_size=128, intermediate_size=256, num_hidden_layers=2, num_attention_heads=2,
+             num_key_value_heads=1, head_dim=64, max_position_embeddings=256)
+    c.update(kw)
+    m = transformers.Qwen3Model(transformers.Qwen3Config(**c)).eval()
+    for p in m.parameters():
+        if p.dim() == 2:
+            p.data.copy_(p.data.bfloat16().float() * 3)
+    return m
+
+
+@pytest.mark.parametrize("kw,what", [
+    ({"attention_bias": True}, "bias"),
+    ({"use_sliding_window": True, "sliding_window": 16, "max_window_layers": 0}, "sliding window"),
+    ({"use_sliding_window": True, "sliding_window": 16, "max_window_layers": 1}, "sliding window"),
+    ({"hidden_act": "gelu"}, "hidden_act"),
+    ({"rope_scaling": {"rope_type": "yarn", "factor": 4.0, "original_max_position_embeddings": 64}}, "rotary"),
+    ({"rope_scaling": {"rope_type": "dynamic", "factor": 2.0}}, "rotary")])
+def test_a_model_that_the_blocks_do_not_compute_is_refused(kw, what):
+    from nano_gpic_b200.models.conditioner import Qwen3TextEncoder
+    from nano_gpic_b200.models.text_lm import TextLM
+    m = _qwen3(**kw)
+    with pytest.raises(ValueError, match=what):
+        TextLM(m)
+    with pytest.raises(ValueError, match=what):
+        Qwen3TextEncoder(model=m, tokenizer=lambda *a, **k: None, native="bf16")
+
+
+@pytest.mark.parametrize("kw", [{}, {"use_sliding_window": True, "sliding_window": 16, "max_window_layers": 2},
+                                {"rope_scaling": {"rope_type": "linear", "factor": 2.0}}])
+def test_what_they_do_compute_is_accepted(kw):
+    """Against transformers in fp32; tolerance as in test_text_lm.py for bf16."""
+    from nano_gpic_b200.models.text_lm import TextLM
+    m = _qwen3(**kw)
+    ids = torch.randint(0, 97, (2, 40), generator=torch.Generator().manual_seed(1))
+    mask = torch.ones_like(ids, dtype=torch.bool)
+    with torch.no_grad():
+        ref = m(input_ids=ids, attention_mask=mask.long())[0]
+    d = TextLM(m).encode(ids, mask).float() - ref
+    assert d.square().mean().sqrt() <= 0.02 * ref.square().mean().sqrt()
