@@ -95,7 +95,8 @@ class Qwen3TextEncoder(BaseConditioner):
     """weight_path: a local Hugging Face Qwen3 directory (tokenizer + model). `model`/`tokenizer` may be given
     directly (e.g. a randomly initialised Qwen3Model from a config, and any callable tokenizer). native="bf16" or "e4m3"
     runs the model on the framework's kernels (models/text_lm.py) with a key/value cache of that type instead of through
-    transformers."""
+    transformers; its projections are a second copy of the model's, laid out at the first caption and again when the
+    module was moved or its weights were replaced."""
 
     def __init__(self, weight_path=None, embed_dim=None, max_length=128, pad_multiple=8, model=None, tokenizer=None,
                  device=None, native=None):
@@ -112,10 +113,24 @@ class Qwen3TextEncoder(BaseConditioner):
         self.embed_dim = embed_dim or self.model.config.hidden_size
         self.max_length, self.pad_multiple = max_length, pad_multiple
         self.null_embedding = None
-        self.native, self.lm = native, None
+        self.native, self._lm, self._lm_of = native, None, None
         if native:
+            from .text_lm import check_model
+            check_model(self.model)
+
+    @property
+    def lm(self):
+        """The model on the framework's kernels (native only), of the module's present weights and device."""
+        if not self.native:
+            return None
+        # a move gives a parameter other memory, a copy into it (load_state_dict) another version
+        now = [(p.device, p.dtype, p.data_ptr(), 0 if p.is_inference() else p._version)
+               for p in self.model.parameters()]
+        if self._lm_of != now:
             from .text_lm import TextLM
-            self.lm = TextLM(self.model)
+            self._lm = None
+            self._lm, self._lm_of = TextLM(self.model), now
+        return self._lm
 
     @property
     def _dev(self):
@@ -136,7 +151,7 @@ class Qwen3TextEncoder(BaseConditioner):
     def encode(self, input_ids, mask):
         dev = self._dev
         input_ids, mask = _to_device(input_ids, dev), _to_device(mask, dev)
-        if self.lm is not None:
+        if self.native:
             out = self.lm.encode(input_ids, mask, kind=self.native)
         else:
             out = self.model(input_ids=input_ids, attention_mask=mask.long())[0]

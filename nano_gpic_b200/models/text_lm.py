@@ -37,7 +37,7 @@ WEIGHTS = tuple(f"{n}.weight" for n in (
 ROPE_TYPES = ("default", "linear", "llama3")
 
 
-def _check_model(model):
+def check_model(model):
     """Raises for what a Qwen3Model may have and the blocks above do not compute."""
     c = model.config
     if set(c.layer_types) != {"full_attention"}:
@@ -48,6 +48,9 @@ def _check_model(model):
     kind = rope.get("rope_type", rope.get("type", "default"))
     if kind not in ROPE_TYPES or getattr(model.rotary_emb, "attention_scaling", 1.0) != 1.0:
         raise ValueError(f"TextLM: rotary embedding of type {ROPE_TYPES} without attention scaling expected, got {kind!r}")
+    rest = sorted(k for k in model.state_dict() if not k.startswith("rotary_emb.") and not k.endswith(WEIGHTS))
+    if rest:
+        raise ValueError(f"TextLM: no use for the model's {rest}")
 
 
 class TextLM:
@@ -57,7 +60,7 @@ class TextLM:
     def __init__(self, model, fp8=None):
         if fp8 not in (None, "mx"):
             raise ValueError(f"fp8 must be None or 'mx', got {fp8!r}")
-        _check_model(model)
+        check_model(model)
         c = model.config
         self.fp8 = fp8
         self.heads, self.kv_heads = c.num_attention_heads, c.num_key_value_heads
@@ -80,9 +83,6 @@ class TextLM:
             up = torch.cat([sd[p + "mlp.gate_proj.weight"], sd[p + "mlp.up_proj.weight"]]).to(BF16)
             w["qkv"], w["up"] = (MXO.quant(qkv), MXO.quant(up)) if fp8 else (qkv, up)
             self.blocks.append(w)
-        rest = sorted(k for k in sd if not k.startswith("rotary_emb.") and not k.endswith(WEIGHTS))
-        if rest:
-            raise ValueError(f"TextLM: no use for the model's {rest}")
 
     def _norm(self, delta, s, w):
         f = N.add_rms_fwd_mx if self.fp8 else N.add_rms_fwd

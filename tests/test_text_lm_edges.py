@@ -45,3 +45,36 @@ def test_what_they_do_compute_is_accepted(kw):
         ref = m(input_ids=ids, attention_mask=mask.long())[0]
     d = TextLM(m).encode(ids, mask).float() - ref
     assert d.square().mean().sqrt() <= 0.02 * ref.square().mean().sqrt()
+
+
+def _captions():
+    ids = torch.randint(0, 97, (3, 24), generator=torch.Generator().manual_seed(2))
+    return ids, torch.arange(24)[None] < torch.tensor([24, 1, 9])[:, None]
+
+
+def _encoder(m, **kw):
+    from nano_gpic_b200.models.conditioner import Qwen3TextEncoder
+    return Qwen3TextEncoder(model=m, tokenizer=lambda *a, **k: None, native="bf16", **kw)
+
+
+def test_native_encoder_follows_the_weights():
+    ids, mask = _captions()
+    enc, other = _encoder(_qwen3()), _qwen3()
+    old, _ = enc.encode(ids, mask)
+    for p in other.parameters():
+        p.data.mul_(1.25)
+    enc.model.load_state_dict(other.state_dict())
+    got, _ = enc.encode(ids, mask)
+    want, _ = _encoder(other).encode(ids, mask)
+    assert torch.equal(got, want) and not torch.equal(got, old)
+    assert enc.lm is enc.lm  # laid out once
+
+
+@pytest.mark.gpu
+def test_native_encoder_follows_the_module_to_another_device():
+    ids, mask = _captions()
+    enc = _encoder(_qwen3())
+    enc.encode(ids, mask)
+    got, _ = enc.to("cuda").encode(ids, mask)
+    want, _ = _encoder(_qwen3(), device="cuda").encode(ids, mask)
+    assert got.is_cuda and torch.equal(got, want)
