@@ -139,6 +139,8 @@ class TextLM:
         """Final hidden states [B, L, hidden] bf16 of a left-aligned batch (zeros where mask is False), the keys and
         values in a cache of `kind`, `chunk` tokens of every sequence at a time (None: all at once)."""
         ids, mask = ids.cpu(), mask.cpu().bool()
+        if (mask[:, 1:] & ~mask[:, :-1]).any():  # the tokens' positions would not be the columns
+            raise ValueError("TextLM: a left-aligned mask expected (each row: its tokens, then padding)")
         lens = mask.sum(1).tolist()
         cache = TextCache(self, len(lens), max(lens + [1]), kind)
         out = torch.zeros(*ids.shape, self.embed.shape[1], dtype=BF16, device=self.device)

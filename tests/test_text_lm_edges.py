@@ -78,3 +78,13 @@ def test_native_encoder_follows_the_module_to_another_device():
     got, _ = enc.to("cuda").encode(ids, mask)
     want, _ = _encoder(_qwen3(), device="cuda").encode(ids, mask)
     assert got.is_cuda and torch.equal(got, want)
+
+
+def test_a_mask_that_is_not_left_aligned_is_refused():
+    from nano_gpic_b200.models.text_lm import TextLM
+    lm = TextLM(_qwen3())
+    ids, mask = _captions()
+    for bad in (mask.flip(1), torch.cat([mask[:, :3], mask[:, :3]], 1) & torch.tensor([1, 0, 1, 1, 1, 1]).bool()):
+        with pytest.raises(ValueError, match="left-aligned"):
+            lm.encode(ids[:, :bad.shape[1]], bad)
+    assert lm.encode(ids[:, :0], mask[:, :0]).shape == (3, 0, 128)
