@@ -395,7 +395,9 @@ std::vector<at::Tensor> paged_attn(const at::Tensor& q, const at::Tensor& pk, co
   check_packed(q, "q", T, q.size(1), pk.device());
   check_i32(total, "total", B, pk.device());
   check_i32(cu, "cu", B + 1, pk.device());
-  TORCH_CHECK(scale > 0 && std::isfinite(scale), "paged: scale must be positive");
+  // as the kernels hold it: a scale that rounds to 0 would make NaN of a masked score, -inf
+  const float scale_log2 = (float)(scale * 1.4426950408889634);
+  TORCH_CHECK(scale_log2 > 0 && std::isfinite(scale_log2), "paged: scale must be positive, in fp32's range");
   TORCH_CHECK(max_new >= 0 && max_total >= 0 && max_new <= INT32_MAX && max_total <= INT32_MAX,
               "paged: max_new / max_total out of range");
   const int64_t H = q.size(1) / D;
@@ -427,7 +429,7 @@ std::vector<at::Tensor> paged_attn(const at::Tensor& q, const at::Tensor& pk, co
   TORCH_CHECK(held <= kMaxTokens, "paged: max_total and the table allow a sequence of too many tokens");
   a.max_total = (int)held;
   a.causal = causal;
-  a.scale_log2 = (float)(scale * 1.4426950408889634);
+  a.scale_log2 = scale_log2;
   a.err = status_word();
   const auto st = at::cuda::getCurrentCUDAStream();
   if (max_new * (H / a.p.Hk) <= rows_max(a.p.ksf != nullptr, B * a.p.Hk))

@@ -154,6 +154,8 @@ def paged_attn(q, cache, table, total, cu, max_new, max_total, scale=None, causa
         scale = 1.0 / math.sqrt(D)
     if not q.is_cuda:
         _check(cache, table, cu, total)
+        if not 1e-45 <= scale <= 2e38:
+            raise RuntimeError("paged: scale must be positive, in fp32's range")
         T, Hk = q.shape[0], cache.k.shape[1]
         H = q.shape[1] // D
         if q.shape[1] % (Hk * D) or H == 0:

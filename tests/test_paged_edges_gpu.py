@@ -176,3 +176,21 @@ def test_second_device_of_a_process(kind):
         there = [x.to("cuda:1") if x is not None else None for x in (q, table, tot, cu, kv.k, kv.v, kv.k_sf, kv.v_sf)]
         got = P.paged_attn(there[0], P.PagedKV(*there[4:]), *there[1:4], n, 200)
         assert all(torch.equal(x, y.to("cuda:0")) for x, y in zip(want, got))
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.1, float("nan"), float("inf"), 1e-50, 1e39])
+def test_scales_that_are_no_positive_fp32_are_refused(scale):
+    from nano_gpic_b200.ops import paged as P
+    kv, table, cu, _, tot = _setup([2, 2], [20, 30], 2, 128, 16, "bf16")
+    with pytest.raises(RuntimeError, match="paged: scale"):
+        P.paged_attn(_q(4, 4, 128), kv, table, tot, cu, 2, 30, scale=scale)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+@pytest.mark.parametrize("n", [1, 150])
+def test_the_least_scale(kind, n):
+    """The smallest scales that pass: every visible key weighs the same, masked ones nothing."""
+    new, total = [n], [400]
+    kv, table, cu, _, _ = _setup(new, total, 2, 128, 16, kind)
+    _fill(kv, table, total)
+    _check(_q(n, 4, 128), kv, table, cu, new, total, scale=1e-44)
