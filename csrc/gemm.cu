@@ -22,6 +22,7 @@
 
 #include "common.cuh"
 #include "gemm.h"
+#include "msg.h"
 #include "status.h"
 
 namespace ng {
@@ -864,14 +865,14 @@ static CUtensorMap make_tmap(const void* ptr, CUtensorMapDataType dt, int esize,
   cuuint32_t estr[3] = {1, 1, 1};
   TORCH_CHECK(ptr != nullptr, "TMA operand is null");
   TORCH_CHECK((reinterpret_cast<uintptr_t>(ptr) & 15) == 0, "TMA base address must be 16-byte aligned");
-  TORCH_CHECK((ld * esize) % 16 == 0, "TMA row stride must be a multiple of 16 bytes, got ld=", ld);
+  TORCH_CHECK((ld * esize) % 16 == 0, msg("TMA row stride must be a multiple of 16 bytes, got ld=", ld));
   TORCH_CHECK(batch == 1 || (bstride * esize) % 16 == 0, "TMA batch stride must be a multiple of 16 bytes");
   NG_TRACE("[tmap] ptr=%p inner=%lld outer=%lld batch=%lld ld=%lld box=%dx%d\n", ptr, (long long)inner,
            (long long)outer, (long long)batch, (long long)ld, box_inner, box_outer);
   CUresult r = get_encode_fn()(&m, dt, 3, const_cast<void*>(ptr), dims, strides, box, estr,
                                CU_TENSOR_MAP_INTERLEAVE_NONE, sw, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  TORCH_CHECK(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled failed: ", (int)r);
+  TORCH_CHECK(r == CUDA_SUCCESS, msg("cuTensorMapEncodeTiled failed: ", (int)r));
   return m;
 }
 
@@ -972,7 +973,7 @@ static void dispatch_epi(int epi, const CUtensorMap& ta, const CUtensorMap& tb, 
     case EPI_GATED: return launch_t<AMN, BMN, EPI_GATED, PAIR>(ta, tb, em, p, tiles, s);
     case EPI_SWIGLU: return launch_t<AMN, BMN, EPI_SWIGLU, PAIR>(ta, tb, em, p, tiles, s);
     case EPI_SWIGLU_BWD: return launch_t<AMN, BMN, EPI_SWIGLU_BWD, PAIR>(ta, tb, em, p, tiles, s);
-    default: TORCH_CHECK(false, "unknown GEMM epilogue ", epi);
+    default: TORCH_CHECK(false, msg("unknown GEMM epilogue ", epi));
   }
 }
 

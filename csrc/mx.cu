@@ -18,6 +18,7 @@
 
 #include "common.cuh"
 #include "gemm.h"
+#include "msg.h"
 #include "status.h"
 
 namespace ng {
@@ -82,7 +83,7 @@ std::vector<at::Tensor> mx_quant(const at::Tensor& x) {
   TORCH_CHECK(x.is_cuda() && x.scalar_type() == at::kBFloat16 && x.dim() == 2 && x.stride(1) == 1,
               "mx_quant: 2-D row-major bf16 CUDA tensor expected");
   const int64_t rows = x.size(0), K = x.size(1);
-  TORCH_CHECK(K % 128 == 0, "mx_quant: K must be a multiple of 128, got ", K);
+  TORCH_CHECK(K % 128 == 0, msg("mx_quant: K must be a multiple of 128, got ", K));
   TORCH_CHECK(x.stride(0) % 8 == 0 && (reinterpret_cast<uintptr_t>(x.data_ptr()) & 15) == 0,
               "mx_quant: 16-byte aligned rows expected");
   const at::cuda::CUDAGuard guard(x.device());
