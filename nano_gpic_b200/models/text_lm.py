@@ -104,6 +104,8 @@ class TextLM:
         dev, D = self.device, self.head_dim
         if len(new) != len(cache.lens) or ids.shape != (sum(new),):
             raise ValueError(f"{len(cache.lens)} counts that add up to the {tuple(ids.shape)} ids expected, got {new}")
+        if min(new, default=0) < 0:
+            raise ValueError(f"counts of new tokens expected, got {new}")
         total = [n + t for n, t in zip(new, cache.lens)]
         if max(total, default=0) > cache.max_tokens:
             raise ValueError(f"a sequence of {max(total)} tokens in a cache of {cache.max_tokens} each")
@@ -141,10 +143,12 @@ class TextLM:
         ids, mask = ids.cpu(), mask.cpu().bool()
         if (mask[:, 1:] & ~mask[:, :-1]).any():  # the tokens' positions would not be the columns
             raise ValueError("TextLM: a left-aligned mask expected (each row: its tokens, then padding)")
+        if chunk is not None and chunk < 1:
+            raise ValueError(f"chunk must be None or positive, got {chunk}")
         lens = mask.sum(1).tolist()
         cache = TextCache(self, len(lens), max(lens + [1]), kind)
         out = torch.zeros(*ids.shape, self.embed.shape[1], dtype=BF16, device=self.device)
-        step = chunk or max(lens + [1])
+        step = max(lens + [1]) if chunk is None else chunk
         for t in range(0, max(lens + [0]), step):
             part = torch.zeros_like(mask)
             part[:, t:t + step] = mask[:, t:t + step]

@@ -88,3 +88,16 @@ def test_a_mask_that_is_not_left_aligned_is_refused():
         with pytest.raises(ValueError, match="left-aligned"):
             lm.encode(ids[:, :bad.shape[1]], bad)
     assert lm.encode(ids[:, :0], mask[:, :0]).shape == (3, 0, 128)
+
+
+def test_negative_counts_and_chunks_are_refused():
+    from nano_gpic_b200.models.text_lm import TextCache, TextLM
+    lm = TextLM(_qwen3())
+    ids, mask = _captions()
+    for chunk in (0, -5):
+        with pytest.raises(ValueError, match="chunk"):
+            lm.encode(ids, mask, chunk=chunk)
+    cache = TextCache(lm, 2, 8)
+    with pytest.raises(ValueError, match="counts"):
+        lm.extend(cache, ids[0, :2], [3, -1])
+    assert cache.lens == [0, 0]
