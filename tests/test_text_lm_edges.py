@@ -101,3 +101,32 @@ def test_negative_counts_and_chunks_are_refused():
     with pytest.raises(ValueError, match="counts"):
         lm.extend(cache, ids[0, :2], [3, -1])
     assert cache.lens == [0, 0]
+
+
+def _at_head_dim_128(dev, kind, chunk, lim):
+    from nano_gpic_b200.models.text_lm import TextLM
+    m = _qwen3(hidden_size=256, num_attention_heads=4, num_key_value_heads=2, head_dim=128)
+    ids = torch.randint(0, 97, (3, 150), generator=torch.Generator().manual_seed(3))
+    mask = torch.arange(150)[None] < torch.tensor([150, 1, 77])[:, None]
+    with torch.no_grad():
+        ref = m(input_ids=ids, attention_mask=mask.long())[0]
+    out = TextLM(m.to(dev)).encode(ids.to(dev), mask.to(dev), kind=kind, chunk=chunk).float().cpu()
+    d, r = (out - ref)[mask], ref[mask]
+    assert (out[~mask] == 0).all() and d.square().mean().sqrt() <= lim * r.square().mean().sqrt()
+
+
+# heads of 128, the encoder's own; tolerances as in test_text_lm.py
+CASES_128 = [("bf16", None, 0.02), ("bf16", 50, 0.02), ("e4m3", None, 0.1)]
+
+
+@pytest.mark.parametrize("kind,chunk,lim", CASES_128)
+def test_head_dim_128_cpu(kind, chunk, lim):
+    _at_head_dim_128("cpu", kind, chunk, lim)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind,chunk,lim", CASES_128 + [("bf16", 1, 0.02), ("e4m3", 8, 0.1)])
+def test_head_dim_128_gpu(kind, chunk, lim):
+    from nano_gpic_b200.ops import status
+    _at_head_dim_128("cuda", kind, chunk, lim)
+    status.check()
