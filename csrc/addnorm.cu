@@ -166,16 +166,16 @@ struct AddRmsBwdArgs {
   int M, C, rows_per_cta;
 };
 
-// A CTA walks its rows, NR at a time; a thread owns VPT vectors of 8 columns for all of them, so the weight gradient's
-// partial sums stay in registers and every byte is read once (a warp per row would read the rows again for the column
-// sums). Bound by bytes and the latency of a row's reduction: the stream's gradient is loaded before the reduction,
-// which takes one barrier (its partial sums alternate between two buffers), and eight CTAs a SM hide it. 32768 x 1024
-// in bf16: 62 us a call, about 10 of them the column sums of the partials (269 MB, 41 us at the copy's rate). NR is 1:
-// two or four rows a step, with more registers and fewer CTAs a SM, took 72 us for the kernel alone. The same loop
-// without NR and the row's bound in its loads ran at 85 us a call with the same 64 registers (measured, not explained).
-template <typename R, int VPT, int NR>
-__global__ void __launch_bounds__(512) add_rms_bwd_kernel(const AddRmsBwdArgs a) {
-  __shared__ float red[2][NR][16];
+// A CTA walks its rows; a thread owns VPT vectors of 8 columns for all of them, so the weight gradient's partial sums
+// stay in registers and every byte is read once. Bound by bytes and the latency of a row's reduction: the stream's
+// gradient is loaded before the reduction, which takes one barrier (its partial sums alternate between two buffers), and
+// eight CTAs a SM hide it. 32768 x 1024 in bf16: 62 us a call, about 10 of them the column sums of the partials (269 MB,
+// 41 us at the copy's rate). Eight CTAs of 128 threads fit a SM at 64 registers: left to itself the compiler takes 73,
+// six CTAs fit, the grid becomes two waves and the call 85 us. Two or four rows a step, with more registers, took 72 us
+// for the kernel alone.
+template <typename R, int VPT>
+__global__ void __launch_bounds__(512, VPT == 1 && sizeof(R) == 2 ? 2 : 0) add_rms_bwd_kernel(const AddRmsBwdArgs a) {
+  __shared__ float red[2][16];
   const int nv = a.C >> 3, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
   const int64_t r0 = (int64_t)blockIdx.x * a.rows_per_cta, r1 = min((int64_t)a.M, r0 + a.rows_per_cta);
   float dw[VPT][8], wf[VPT][8];
@@ -187,64 +187,51 @@ __global__ void __launch_bounds__(512) add_rms_bwd_kernel(const AddRmsBwdArgs a)
     if (v < nv) load8(a.w + v * 8, wf[i]);
   }
   int buf = 0;
-  for (int64_t row = r0; row < r1; row += NR, buf ^= 1) {
-    float g[NR][VPT][8], xn[NR][VPT][8], rs[NR], acc[NR];
-    Raw<R> ds[NR][VPT];
+  for (int64_t row = r0; row < r1; ++row, buf ^= 1) {
+    float g[VPT][8], xn[VPT][8];
+    Raw<R> ds[VPT];
+    const float rs = a.rstd[row];
 #pragma unroll
-    for (int n = 0; n < NR; ++n) {
-      const bool live = row + n < r1;
-      rs[n] = live ? a.rstd[row + n] : 0.f;
+    for (int i = 0; i < VPT; ++i) {
+      const int v = threadIdx.x + i * blockDim.x;
+      if (v < nv) {
+        load8(a.dh + row * a.lddh + v * 8, g[i]);
+        load8(static_cast<const R*>(a.s) + row * a.lds + v * 8, xn[i]);
+        if (a.ds != nullptr) ds[i].load(static_cast<const R*>(a.ds) + row * a.ldds + v * 8);
+      } else {
 #pragma unroll
-      for (int i = 0; i < VPT; ++i) {
-        const int v = threadIdx.x + i * blockDim.x;
-        if (live && v < nv) {
-          load8(a.dh + (row + n) * a.lddh + v * 8, g[n][i]);
-          load8(static_cast<const R*>(a.s) + (row + n) * a.lds + v * 8, xn[n][i]);
-          if (a.ds != nullptr) ds[n][i].load(static_cast<const R*>(a.ds) + (row + n) * a.ldds + v * 8);
-        } else {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) g[n][i][j] = xn[n][i][j] = 0.f;
-        }
+        for (int j = 0; j < 8; ++j) g[i][j] = xn[i][j] = 0.f;
       }
     }
+    float acc = 0.f;
 #pragma unroll
-    for (int n = 0; n < NR; ++n) {
-      acc[n] = 0.f;
+    for (int i = 0; i < VPT; ++i)
 #pragma unroll
-      for (int i = 0; i < VPT; ++i)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          xn[n][i][j] *= rs[n];
-          dw[i][j] += g[n][i][j] * xn[n][i][j];
-          g[n][i][j] *= wf[i][j];
-          acc[n] += g[n][i][j] * xn[n][i][j];
-        }
-      acc[n] = warp_sum(acc[n]);
-      if (nw > 1 && (threadIdx.x & 31) == 0) red[buf][n][warp] = acc[n];
-    }
+      for (int j = 0; j < 8; ++j) {
+        xn[i][j] *= rs;
+        dw[i][j] += g[i][j] * xn[i][j];
+        g[i][j] *= wf[i][j];
+        acc += g[i][j] * xn[i][j];
+      }
+    acc = warp_sum(acc);
     if (nw > 1) {
+      if ((threadIdx.x & 31) == 0) red[buf][warp] = acc;
       __syncthreads();
-#pragma unroll
-      for (int n = 0; n < NR; ++n) {
-        acc[n] = 0.f;
-        for (int k = 0; k < nw; ++k) acc[n] += red[buf][n][k];
-      }
+      acc = 0.f;
+      for (int k = 0; k < nw; ++k) acc += red[buf][k];
     }
+    const float cm = acc / (float)a.C;
 #pragma unroll
-    for (int n = 0; n < NR; ++n) {
-      const float cm = acc[n] / (float)a.C;
+    for (int i = 0; i < VPT; ++i) {
+      const int v = threadIdx.x + i * blockDim.x;
+      if (v < nv) {
+        float o[8];
 #pragma unroll
-      for (int i = 0; i < VPT; ++i) {
-        const int v = threadIdx.x + i * blockDim.x;
-        if (row + n < r1 && v < nv) {
-          float o[8];
+        for (int j = 0; j < 8; ++j) o[j] = 0.f;
+        if (a.ds != nullptr) ds[i].get(o);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) o[j] = 0.f;
-          if (a.ds != nullptr) ds[n][i].get(o);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) o[j] += rs[n] * (g[n][i][j] - xn[n][i][j] * cm);
-          store8(static_cast<R*>(a.dx) + (row + n) * a.C + v * 8, o);
-        }
+        for (int j = 0; j < 8; ++j) o[j] += rs * (g[i][j] - xn[i][j] * cm);
+        store8(static_cast<R*>(a.dx) + row * a.C + v * 8, o);
       }
     }
   }
@@ -402,11 +389,11 @@ at::Tensor add_rms_bwd(const at::Tensor& dh, const c10::optional<at::Tensor>& ds
   const auto st = at::cuda::getCurrentCUDAStream();
 #define NG_ADD_RMS_BWD(R)                                           \
   if (vpt == 1)                                                     \
-    add_rms_bwd_kernel<R, 1, 1><<<grid, threads, 0, st>>>(a);       \
+    add_rms_bwd_kernel<R, 1><<<grid, threads, 0, st>>>(a);       \
   else if (vpt == 2)                                                \
-    add_rms_bwd_kernel<R, 2, 1><<<grid, threads, 0, st>>>(a);       \
+    add_rms_bwd_kernel<R, 2><<<grid, threads, 0, st>>>(a);       \
   else                                                              \
-    add_rms_bwd_kernel<R, 4, 1><<<grid, threads, 0, st>>>(a)
+    add_rms_bwd_kernel<R, 4><<<grid, threads, 0, st>>>(a)
   if (f32) {
     NG_ADD_RMS_BWD(float);
   } else {
