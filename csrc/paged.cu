@@ -120,14 +120,6 @@ __global__ void __launch_bounds__(256) cache_write_kernel(const CopyArgs a) {
   }
 }
 
-// four e4m3 bytes times a power of two -> four bf16 (exact: e4m3 has 4 significant bits)
-__device__ __forceinline__ uint2 e4m3_to_bf16(uint32_t w, float s) {
-  const __half2 lo = __half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w & 0xFFFFu), __NV_E4M3));
-  const __half2 hi = __half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w >> 16), __NV_E4M3));
-  const float2 a = __half22float2(lo), b = __half22float2(hi);
-  return make_uint2(pack_bf16(a.x * s, a.y * s), pack_bf16(b.x * s, b.y * s));
-}
-
 // The inverse: the loads of four units a group are issued before the first is converted and stored. 70,000 tokens of
 // 8 heads of 128 out of e4m3 pages: 84 us, 5.2 TB/s (one unit at a time, a lookup for each: 110 us).
 template <int D, bool Q8>
@@ -174,7 +166,7 @@ __global__ void __launch_bounds__(256) cache_read_kernel(const CopyArgs a) {
         uint4 u = kv[x][c];
         if (Q8) {
           const float s = ldexpf(1.f, (int)sf[x][c] - 127);
-          const uint2 lo = e4m3_to_bf16(u.x, s), hi = e4m3_to_bf16(u.y, s);
+          const uint2 lo = e4m3x4_bf16x4(u.x, s), hi = e4m3x4_bf16x4(u.y, s);
           u = make_uint4(lo.x, lo.y, hi.x, hi.y);
         }
         __stcs(reinterpret_cast<uint4*>((c ? a.v : a.k) + (r0 + i[x]) * (c ? a.ldv : a.ldk) + h[x] * D + l * 8), u);

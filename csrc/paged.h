@@ -6,9 +6,12 @@
 #pragma once
 #include <c10/cuda/CUDAException.h>
 #include <cuda_bf16.h>
+#include <cuda_fp16.h>
 #include <stdint.h>
 
 #include <mutex>
+
+#include "common.cuh"
 
 namespace ng {
 
@@ -28,6 +31,30 @@ struct PagedPool {
 // Scale exponents are kept in [kScaleLo, kScaleHi]: the ratio of two scales and of their products with probabilities
 // then stays inside fp32's normal range (values beyond 448 * 2^63 saturate, values below 2^-71 round to zero).
 constexpr int kScaleLo = -62, kScaleHi = 63;
+
+__device__ __forceinline__ float exp2i(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }  // |e| <= 126
+
+// two e4m3 bytes (the low half of w) -> f16x2, exact
+__device__ __forceinline__ uint32_t e4m3x2_f16x2(uint32_t w) {
+  uint32_t r;
+  asm("{\n\t.reg .b16 lo;\n\tcvt.u16.u32 lo, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t}\n" : "=r"(r) : "r"(w));
+  return r;
+}
+// four e4m3 bytes times a power of two -> two bf16x2, exact (e4m3 has 4 significant bits)
+__device__ __forceinline__ uint2 e4m3x4_bf16x4(uint32_t w, float f) {
+  uint32_t a, b;
+  asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %2;\n\t"
+      "cvt.rn.f16x2.e4m3x2 %0, lo;\n\tcvt.rn.f16x2.e4m3x2 %1, hi;\n\t}\n"
+      : "=r"(a), "=r"(b)
+      : "r"(w));
+  const float2 x = __half22float2(*reinterpret_cast<__half2*>(&a)), y = __half22float2(*reinterpret_cast<__half2*>(&b));
+  return make_uint2(pack_bf16(x.x * f, x.y * f), pack_bf16(y.x * f, y.y * f));
+}
+
+// 16 bytes to shared memory, zeros where not live
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool live) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
+}
 
 // First row of (page, head) in units of tokens; 64-bit, a pool may hold more than 2^31 elements.
 __device__ __forceinline__ int64_t paged_row(const PagedPool& p, int pg, int head, int slot) {

@@ -25,8 +25,6 @@
 #include <ATen/cuda/CUDAContext.h>
 #include <torch/extension.h>
 
-#include <cuda_fp16.h>
-
 #include "common.cuh"
 #include "paged.h"
 #include "status.h"
@@ -59,9 +57,6 @@ struct Tile {
   }
 };
 
-__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool live) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
-}
 __device__ __forceinline__ void cp4(uint32_t dst, const void* src, bool live) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(live ? 4 : 0) : "memory");
 }
@@ -93,12 +88,6 @@ __device__ __forceinline__ void mma16(float (&d)[4], const uint32_t (&a)[4], uin
         "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-// two e4m3 bytes (the low half of w) -> f16x2, exact
-__device__ __forceinline__ uint32_t e4m3x2_f16x2(uint32_t w) {
-  uint32_t r;
-  asm("{\n\t.reg .b16 lo;\n\tcvt.u16.u32 lo, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t}\n" : "=r"(r) : "r"(w));
-  return r;
 }
 __device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
   __half2 h = __floats2half2_rn(lo, hi);
@@ -132,7 +121,6 @@ __device__ __forceinline__ float quad_sum(float v) {
   v += __shfl_xor_sync(0xffffffffu, v, 1);
   return v + __shfl_xor_sync(0xffffffffu, v, 2);
 }
-__device__ __forceinline__ float exp2i(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }  // |e| <= 126
 
 }  // namespace
 
@@ -240,8 +228,8 @@ __global__ void __launch_bounds__(kWarps * 32, 2) paged_rows_kernel(const PagedA
       const bool live = row >= 0;
       const int64_t src = (live ? row : 0) * T::RB + col * 16;
       const uint32_t dst = st + T::off(r, col);
-      cp16(dst, static_cast<const uint8_t*>(a.p.k) + src, live);
-      cp16(dst + kStageBytes / 2, static_cast<const uint8_t*>(a.p.v) + src, live);
+      cp_async16(dst, static_cast<const uint8_t*>(a.p.k) + src, live);
+      cp_async16(dst + kStageBytes / 2, static_cast<const uint8_t*>(a.p.v) + src, live);
     }
     if (Q8) {  // scale bytes, four tokens a copy (pages are multiples of eight tokens)
       const int r = (lane * 4) % KT;

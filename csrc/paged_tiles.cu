@@ -33,8 +33,6 @@
 #include <ATen/cuda/CUDAContext.h>
 #include <torch/extension.h>
 
-#include <cuda_fp16.h>
-
 #include "common.cuh"
 #include "gemm.h"
 #include "paged.h"
@@ -64,26 +62,11 @@ struct Lay {
   static constexpr int SMEM = TAB + (2048 + 4) * 4 + 1024;
 };
 
-__device__ __forceinline__ float exp2i(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }  // |e| <= 126
-
-// four e4m3 bytes times a power of two -> two bf16x2, exact
-__device__ __forceinline__ uint2 e4m3x4_bf16x4(uint32_t w, float f) {
-  uint32_t a, b;
-  asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %2;\n\t"
-      "cvt.rn.f16x2.e4m3x2 %0, lo;\n\tcvt.rn.f16x2.e4m3x2 %1, hi;\n\t}\n"
-      : "=r"(a), "=r"(b)
-      : "r"(w));
-  const float2 x = __half22float2(*reinterpret_cast<__half2*>(&a)), y = __half22float2(*reinterpret_cast<__half2*>(&b));
-  return make_uint2(pack_bf16(x.x * f, x.y * f), pack_bf16(y.x * f, y.y * f));
-}
 // byte offset of 16-byte chunk c of row r in a tile of 64-column atoms with the 128-byte swizzle
 __device__ __forceinline__ int tile_off(int r, int c) {
   return (c >> 3) * kAtom + r * 128 + (((c & 7) ^ (r & 7)) << 4);
 }
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool live) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
-}
 __device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
 // D[tmem] (+)= A B^T with descriptors given as halves (the upper half a constant): A from shared memory, or from TMEM.
@@ -563,36 +546,35 @@ __global__ void __launch_bounds__(kThreads, 1)
     regs_less<kRegsRest<Q8>>();
     if (warp == 15) {
       // ----------------------------------------------------------------------------------------------------- pieces
-    if (lane == 0) {
-      Pieces pieces(t, tab);
-      for (uint32_t k = 0;; ++k) {
-        const Piece p = pieces.next();
-        if (!mbar_wait(&d_empty[k % kRing], ((k / kRing) & 1) ^ 1, abort_flag, a.err, kErrWaitEmpty)) break;
-        ring[k % kRing] = p;
-        mbar_arrive(&d_full[k % kRing]);
-        if (!p.valid) break;
-      }
-      if (t.cuts != nullptr) {  // for the merge
-        const int c = blockIdx.x, ctas = gridDim.x, u = share_start(t, tab, c, ctas);
-        int* out = t.cuts + c * 8;
-        Cut cut = {0, 0, 0, 0, c};
-        if (u < tab[t.entries]) {
-          const Place p = place_of(t, tab, u);
-          if (p.off > 0 && share_start(t, tab, c - 1, ctas) <= p.item) {
-            const Entry w = entry_of(a, p.e);
-            cut = {w.row0, w.r0, w.rows, (p.item - tab[p.e]) / p.cost, c};
-            while (cut.last + 1 < ctas && share_start(t, tab, cut.last + 1, ctas) < p.item + p.cost) ++cut.last;
-          }
+      if (lane == 0) {
+        Pieces pieces(t, tab);
+        for (uint32_t k = 0;; ++k) {
+          const Piece p = pieces.next();
+          if (!mbar_wait(&d_empty[k % kRing], ((k / kRing) & 1) ^ 1, abort_flag, a.err, kErrWaitEmpty)) break;
+          ring[k % kRing] = p;
+          mbar_arrive(&d_full[k % kRing]);
+          if (!p.valid) break;
         }
-        out[0] = u, out[1] = cut.row0, out[2] = cut.r0, out[3] = cut.rows, out[4] = cut.hk, out[5] = cut.last;
-        out[6] = share_start(t, tab, c + 1, ctas);
+        if (t.cuts != nullptr) {  // for the merge
+          const int c = blockIdx.x, ctas = gridDim.x, u = share_start(t, tab, c, ctas);
+          int* out = t.cuts + c * 8;
+          Cut cut = {0, 0, 0, 0, c};
+          if (u < tab[t.entries]) {
+            const Place p = place_of(t, tab, u);
+            if (p.off > 0 && share_start(t, tab, c - 1, ctas) <= p.item) {
+              const Entry w = entry_of(a, p.e);
+              cut = {w.row0, w.r0, w.rows, (p.item - tab[p.e]) / p.cost, c};
+              while (cut.last + 1 < ctas && share_start(t, tab, cut.last + 1, ctas) < p.item + p.cost) ++cut.last;
+            }
+          }
+          out[0] = u, out[1] = cut.row0, out[2] = cut.r0, out[3] = cut.rows, out[4] = cut.hk, out[5] = cut.last;
+          out[6] = share_start(t, tab, c + 1, ctas);
+        }
       }
-    }
     } else if (warp == 14) {
       if (Q8) load_q(0);
     } else {
       // ------------------------------------------------------------------------------------------------- MMA issue
-    {
       constexpr uint32_t idesc_s = idesc_bf16_f32(kTileRows, kHalf, 0, 0);
       constexpr uint32_t idesc_o = idesc_bf16_f32(kTileRows, D, 0, 1);
       // A warp per row tile, so that one's bookkeeping runs under the other's products: descriptors are a constant
@@ -602,75 +584,72 @@ __global__ void __launch_bounds__(kThreads, 1)
       constexpr uint32_t lbo = (uint32_t)(kAtom >> 4) << 16;                    // between V's 64-column atoms
       const uint32_t q_lo = (smem_u32(smem + L::Q) >> 4) | (1u << 16), k_lo = (smem_u32(smem + L::K) >> 4) | (1u << 16);
       const uint32_t v_lo = (smem_u32(smem + L::V) >> 4) | lbo;
-      {
-        const int X = warp - 12;
-        const uint32_t q_x = q_lo + X * (L::TB >> 4), s_x = tmem + C_S + X * kKeys, o_x = tmem + C_O + X * D;
-        uint32_t g = 0, q = 0;      // key tiles of this CTA before the piece (ring position), pieces
-        uint32_t pp = 0;            // phase bits of p_full, per half
-        uint32_t outs = 0;          // outputs finished
-        bool ok = true;
-        while (ok && take()) {
-          const int n = s.j1 - s.j0;
-          if (n <= 0) continue;
-          const bool live_b = s.rows > kTileRows;
-          const int all = min(2 * n, (s.kend - s.j0 * kKeys + kHalf - 1) / kHalf);  // halves of the piece
-          const int mine = X == 1 ? (live_b ? all : 0) : (live_b ? max(0, min(all, s.ja - 2 * s.j0)) : all);
-          const uint32_t qb = q % L::QB, qd = q_x + qb * 2 * (L::TB >> 4);
-          ok = wait_all(&q_full[qb], (q / L::QB) & 1, kErrWaitFull);
-          ++q;
+      const int X = warp - 12;
+      const uint32_t q_x = q_lo + X * (L::TB >> 4), s_x = tmem + C_S + X * kKeys, o_x = tmem + C_O + X * D;
+      uint32_t g = 0, q = 0;      // key tiles of this CTA before the piece (ring position), pieces
+      uint32_t pp = 0;            // phase bits of p_full, per half
+      uint32_t outs = 0;          // outputs finished
+      bool ok = true;
+      while (ok && take()) {
+        const int n = s.j1 - s.j0;
+        if (n <= 0) continue;
+        const bool live_b = s.rows > kTileRows;
+        const int all = min(2 * n, (s.kend - s.j0 * kKeys + kHalf - 1) / kHalf);  // halves of the piece
+        const int mine = X == 1 ? (live_b ? all : 0) : (live_b ? max(0, min(all, s.ja - 2 * s.j0)) : all);
+        const uint32_t qb = q % L::QB, qd = q_x + qb * 2 * (L::TB >> 4);
+        ok = wait_all(&q_full[qb], (q / L::QB) & 1, kErrWaitFull);
+        ++q;
 #pragma unroll 1
-          for (int u = 0; ok && u < all + 2; ++u) {
-            const uint32_t h = u & 1, hs = s_x + h * kHalf;
-            const bool ends = h == 1;
-            // O += P V of half u - 2
-            if (u >= 2) {
-              const int v = u - 2;
-              const uint32_t gg = g + (v >> 1), st = gg & 1;
-              if (v < mine) {
-                if (h == 0) ok = wait_all(&v_full[st], (gg >> 1) & 1, kErrWaitFull);
-                ok = ok && wait_all(&p_full[X * 2 + h], (pp >> h) & 1, kErrWaitFull);
-                pp ^= 1u << h;
-                // the piece's first product overwrites O: the previous piece's output has been read
-                if (v == 0 && outs > 0) ok = ok && wait_all(&o_empty[X], (outs - 1) & 1, kErrWaitAccEmpty);
-                if (!ok) break;
-                tc_fence_after();
-                const uint32_t vd = v_lo + st * (L::TB >> 4) + h * (kHalf * 128 >> 4);
-#pragma unroll
-                for (int k = 0; k < kHalf / 16; ++k)
-                  umma_ts(o_x, hs + k * 8, vd + k * (2048 >> 4), hi, idesc_o, (k != 0 || v != 0) ? 1u : 0u);
-                umma_commit_elect(&pv_done[X * 2 + h]);
-                if (v + 1 == mine) ++outs;
-              } else if (ends || v + 1 == all) {  // a tile this one does not see is released once it is there
-                if (mine <= (v & ~1)) ok = wait_all(&v_full[st], (gg >> 1) & 1, kErrWaitFull);
-              }
-              if (ends || v + 1 == all) umma_commit_elect(&v_empty[st]);
-            }
-            // S of half u (its buffer: P V of half u - 2, issued before, has read P there)
-            if (u < all) {
-              const uint32_t gg = g + (u >> 1), st = gg & 1;
-              if (h == 0) ok = ok && wait_all(&k_full[st], (gg >> 1) & 1, kErrWaitFull);
+        for (int u = 0; ok && u < all + 2; ++u) {
+          const uint32_t h = u & 1, hs = s_x + h * kHalf;
+          const bool ends = h == 1;
+          // O += P V of half u - 2
+          if (u >= 2) {
+            const int v = u - 2;
+            const uint32_t gg = g + (v >> 1), st = gg & 1;
+            if (v < mine) {
+              if (h == 0) ok = wait_all(&v_full[st], (gg >> 1) & 1, kErrWaitFull);
+              ok = ok && wait_all(&p_full[X * 2 + h], (pp >> h) & 1, kErrWaitFull);
+              pp ^= 1u << h;
+              // the piece's first product overwrites O: the previous piece's output has been read
+              if (v == 0 && outs > 0) ok = ok && wait_all(&o_empty[X], (outs - 1) & 1, kErrWaitAccEmpty);
               if (!ok) break;
-              if (u < mine) {
-                const uint32_t kd = k_lo + st * (L::TB >> 4) + h * (kHalf * 128 >> 4);
+              tc_fence_after();
+              const uint32_t vd = v_lo + st * (L::TB >> 4) + h * (kHalf * 128 >> 4);
 #pragma unroll
-                for (int k = 0; k < D / 16; ++k) {
-                  const uint32_t off = (k >> 2) * (kAtom >> 4) + (k & 3) * (32 >> 4);
-                  umma_ss(hs, qd + off, kd + off, hi, idesc_s, k != 0 ? 1u : 0u);
-                }
-                umma_commit_elect(&s_full[X * 2 + h]);
-              }
-              if (ends || u + 1 == all) umma_commit_elect(&k_empty[st]);
-              if (u + 1 == all) umma_commit_elect(&q_empty[qb]);
+              for (int k = 0; k < kHalf / 16; ++k)
+                umma_ts(o_x, hs + k * 8, vd + k * (2048 >> 4), hi, idesc_o, (k != 0 || v != 0) ? 1u : 0u);
+              umma_commit_elect(&pv_done[X * 2 + h]);
+              if (v + 1 == mine) ++outs;
+            } else if (ends || v + 1 == all) {  // a tile this one does not see is released once it is there
+              if (mine <= (v & ~1)) ok = wait_all(&v_full[st], (gg >> 1) & 1, kErrWaitFull);
             }
+            if (ends || v + 1 == all) umma_commit_elect(&v_empty[st]);
           }
-          g += n;
+          // S of half u (its buffer: P V of half u - 2, issued before, has read P there)
+          if (u < all) {
+            const uint32_t gg = g + (u >> 1), st = gg & 1;
+            if (h == 0) ok = ok && wait_all(&k_full[st], (gg >> 1) & 1, kErrWaitFull);
+            if (!ok) break;
+            if (u < mine) {
+              const uint32_t kd = k_lo + st * (L::TB >> 4) + h * (kHalf * 128 >> 4);
+#pragma unroll
+              for (int k = 0; k < D / 16; ++k) {
+                const uint32_t off = (k >> 2) * (kAtom >> 4) + (k & 3) * (32 >> 4);
+                umma_ss(hs, qd + off, kd + off, hi, idesc_s, k != 0 ? 1u : 0u);
+              }
+              umma_commit_elect(&s_full[X * 2 + h]);
+            }
+            if (ends || u + 1 == all) umma_commit_elect(&k_empty[st]);
+            if (u + 1 == all) umma_commit_elect(&q_empty[qb]);
+          }
         }
-        if (!ok || *abort_flag) {  // products in flight finish before TMEM is released
-          umma_commit_elect(&drain[X]);
-          mbar_drain(&drain[X], 0);
-        }
+        g += n;
       }
-    }
+      if (!ok || *abort_flag) {  // products in flight finish before TMEM is released
+        umma_commit_elect(&drain[X]);
+        mbar_drain(&drain[X], 0);
+      }
     }
   } else {
     // ---------------------------------------------------------------------------------------------------- softmax
