@@ -107,14 +107,14 @@ struct PagedAttnArgs {
 constexpr int kSMs = 148;
 constexpr int kMaxTokens = INT32_MAX - 8192;  // of a sequence: positions a tile past the end stay inside an int
 
-// Tokens of a sequence with n new rows, its entry in `total` given, that the kernels work on. The status word is set
-// where it is beyond the caller's bound, or beyond what its row of the table holds.
-__device__ __forceinline__ int paged_total(const PagedAttnArgs& a, int n, int total) {
-  if (total > a.bound_total)
+// Sets the status word where sequence b is beyond the caller's bounds, or beyond what its row of the table holds; what
+// follows works on rows and tokens cut down to the launch's. Once a sequence and launch.
+__device__ __forceinline__ void paged_check(const PagedAttnArgs& a, int b) {
+  const int n = min(__ldg(a.cu + b + 1), a.T) - max(0, __ldg(a.cu + b)), total = __ldg(a.total + b);
+  if (n > a.bound_new || total > a.bound_total)
     raise_error(a.err, kErrBound);
   else if (n > 0 && total > a.max_total)
     raise_error(a.err, kErrPage);
-  return max(0, min(total, a.max_total));
 }
 
 // Allows a kernel `bytes` of dynamic shared memory, once a device: the attribute belongs to the function on the current

@@ -141,8 +141,8 @@ __global__ void __launch_bounds__(kWarps * 32, 2) paged_rows_kernel(const PagedA
   const int G = a.H / a.p.Hk;
   const int row0 = max(0, __ldg(a.cu + b));
   const int n = max(0, min(__ldg(a.cu + b + 1), a.T) - row0);
-  if (n > a.bound_new && threadIdx.x == 0) raise_error(a.err, kErrBound);
-  const int total = paged_total(a, n, __ldg(a.total + b));
+  if (threadIdx.x == 0 && split == 0 && rt == 0 && hk == 0) paged_check(a, b);
+  const int total = max(0, min(__ldg(a.total + b), a.max_total));
   const int R = min(kRows, n * G - rt * kRows);  // rows of this tile; row r: token (rt * 16 + r) / G, head hk G + rest
   if (R <= 0) return;
   const int used = paged_used_splits(a, total);

@@ -155,8 +155,7 @@ __device__ __forceinline__ Entry entry_of(const PagedAttnArgs& a, int e) {
   w.r0 = (e - w.b * a.row_tiles) * 2 * kTileRows;
   w.row0 = max(0, __ldg(a.cu + w.b));
   w.n = max(0, min(__ldg(a.cu + w.b + 1), a.T) - w.row0);
-  if (w.n > a.bound_new) raise_error(a.err, kErrBound);
-  w.total = paged_total(a, w.n, __ldg(a.total + w.b));
+  w.total = max(0, min(__ldg(a.total + w.b), a.max_total));
   w.rows = max(0, min(2 * kTileRows, w.n * G - w.r0));
   auto seen = [&](int r) { return a.causal ? max(0, min(w.total, w.total - w.n + r / G + 1)) : w.total; };
   w.kend = w.rows > 0 ? seen(w.r0 + w.rows - 1) : 0;
@@ -340,6 +339,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
   }
+  for (int b = blockIdx.x * kThreads + threadIdx.x; b < a.B; b += gridDim.x * kThreads) paged_check(a, b);
   if (t.balanced) cost_table(t, tab, warp_sums);
   tc_fence_before();
   __syncthreads();
