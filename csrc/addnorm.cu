@@ -91,9 +91,10 @@ struct AddRmsArgs {
 };
 
 // One CTA per row, VPT vectors of 8 columns a thread, held in registers between the sum and the output: one read of x
-// and of the stream, one write of each output. Bound by bytes where rows are many (20480 x 2048 to MXFP8: 52 us, 5.7
-// TB/s; 4099 x 5120 with an fp32 stream: 43 us, 5.9 TB/s), by the launch and the call where they are few (16 x 2048:
-// 10 us a call). One vector a thread up to 4096 columns: the most loads in flight a row and the fewest registers.
+// and of the stream, one write of each output. Bound by bytes where rows are many (20480 x 2048 to MXFP8: 56 us a
+// call, 5.3 TB/s; 4099 x 5120 with an fp32 stream: 43 us, 5.9 TB/s), by the launch and the call where they are few
+// (16 x 2048: 10 us a call). One vector a thread up to 4096 columns: the most loads in flight a row and the fewest
+// registers.
 template <typename R, bool MXO, int VPT>
 __global__ void __launch_bounds__(512) add_rms_fwd_kernel(const AddRmsArgs a) {
   __shared__ float red[32];
@@ -168,11 +169,11 @@ struct AddRmsBwdArgs {
 
 // A CTA walks its rows; a thread owns VPT vectors of 8 columns for all of them, so the weight gradient's partial sums
 // stay in registers and every byte is read once. Bound by bytes and the latency of a row's reduction: the stream's
-// gradient is loaded before the reduction, which takes one barrier (its partial sums alternate between two buffers), and
-// eight CTAs a SM hide it. 32768 x 1024 in bf16: 62 us a call, about 10 of them the column sums of the partials (269 MB,
-// 41 us at the copy's rate). Eight CTAs of 128 threads fit a SM at 64 registers: left to itself the compiler takes 73,
-// six CTAs fit, the grid becomes two waves and the call 85 us. Two or four rows a step, with more registers, took 72 us
-// for the kernel alone.
+// gradient is loaded before the reduction, which takes one barrier (its partial sums alternate between two buffers),
+// and eight CTAs a SM hide it. 32768 x 1024 in bf16: 62 us a call, about 10 of them the column sums of the partials
+// (269 MB, 41 us at the copy's rate). Eight CTAs of 128 threads fit a SM at 64 registers: left to itself the compiler
+// takes 73, six CTAs fit, the grid becomes two waves and the call 85 us. Two or four rows a step, with more
+// registers, took 72 us for the kernel alone.
 template <typename R, int VPT>
 __global__ void __launch_bounds__(512, VPT == 1 && sizeof(R) == 2 ? 2 : 0) add_rms_bwd_kernel(const AddRmsBwdArgs a) {
   __shared__ float red[2][16];

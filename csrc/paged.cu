@@ -218,8 +218,11 @@ __global__ void __launch_bounds__(256) paged_merge_kernel(const PagedAttnArgs a)
 // further. Both measured, us, 8 key heads of 128 (row / tile kernel):
 //   bf16   16 rows: 1 x 8192 keys 26 / 50, 64 x 8192 346 / 402;   32 rows: 1 x 8192 28 / 52, 8 x 512 16 / 21,
 //          8 x 8192 91 / 82, 64 x 8192 478 / 404: 32 rows pay while the key heads of all sequences leave SMs idle
-//   e4m3   32 rows: 1 x 8192 26 / 66, 8 x 8192 79 / 158, 64 x 8192 431 / 998 (the tile kernel converts the tiles); 16
-//          more rows cost the row kernel 200, so it stays ahead to 64
+//   e4m3   32 rows: 1 x 8192 28 / 65, 8 x 8192 85 / 159, 64 x 8192 456 / 1009; 64 rows: 38 / 67, 128 / 159, 884 / 1015
+//          (the tile kernel converts the tiles); 96 rows: tile kernel 69, 165, 1025, where another 200 for each 16 rows
+//          of the row kernel would pass it at 64 x 8192
+// Heads of 64: bf16, 16 rows: 1 x 8192 19 / 50, 64 x 8192 192 / 386; 32 rows: 8 x 8192 56 / 73; e4m3, 64 rows: 28 / 58,
+// 85 / 116, 566 / 693.
 inline int64_t rows_max(bool q8, int64_t heads) { return q8 ? 64 : heads < kSMs / 2 ? 32 : 16; }
 
 bool opt(const c10::optional<at::Tensor>& t) { return t.has_value() && t->defined(); }

@@ -142,8 +142,8 @@ __device__ __forceinline__ int paged_used_splits(const PagedAttnArgs& a, int tot
   return max(1, (total + a.split_len - 1) / a.split_len);
 }
 
-// A row, or a part of it, that saw no key has m = -inf and l = 0. A NaN score moves no maximum (fmaxf drops it) but makes
-// the sum NaN, so m alone does not tell: the sum decides, here and in every merge.
+// A row, or a part of it, that saw no key has m = -inf and l = 0. A NaN score moves no maximum (fmaxf drops it) but
+// makes the sum NaN, so m alone does not tell: the sum decides, here and in every merge.
 __device__ __forceinline__ bool paged_saw_nothing(float m, float l) { return m == -INFINITY && l == 0.f; }
 
 // log-sum-exp (natural) of a row from its maximum (log2 units) and its sum relative to it; NaN where the sum is

@@ -9,19 +9,21 @@
 // flight; no CTA barrier in the loop), with its own running maximum and sum in fp32. The four warps, then the splits,
 // are merged by their maxima in a fixed order (csrc/paged.cu, paged_merge_kernel).
 //
-// e4m3 pools: an e4m3 value is exact in f16, so the products run in f16 on the stored bytes, unscaled. The row of Q is
-// brought to [2^14, 2^15) by a power of two first (exact but for values 2^-29 below the row's largest). The key's
+// e4m3 pools: an e4m3 value is exact in f16, so the products run in f16 on the stored bytes, unscaled. The row of Q
+// is brought to [2^14, 2^15) by a power of two first (exact but for values 2^-29 below the row's largest). The key's
 // scale multiplies the fp32 score; the value's, 2^e, enters the exponent: w = 2^(s + e - M), o = sum w v8, l = sum w
 // 2^-e, with M the running maximum of s + e, less 15: weights reach 2^15. P is rounded to f16 (bf16 pools: bf16, the
-// type of V) for its product; the row sum keeps the unrounded fp32 values. One token can lie far above the others in s +
-// e and still add nothing to a column (a zero value, whose scale is 1, or a single loud channel), so weights of any size
-// must keep their bits: where a tile has weights below 2^-16 (the least that f16 rounds as finely as bf16), what the
-// rounding left of them is multiplied again, 2^40 up, into accumulators that are scaled along.
+// type of V) for its product; the row sum keeps the unrounded fp32 values. One token can lie far above the others in
+// s + e and still add nothing to a column (a zero value, whose scale is 1, or a single loud channel), so weights of
+// any size must keep their bits: where a tile has weights below 2^-16 (the least that f16 rounds as finely as bf16),
+// what the rounding left of them is multiplied again, 2^40 up, into accumulators that are scaled along.
 //
-// One step of 64 sequences of up to 16384 tokens, 8 key heads of 128, e4m3 (1.34 GB): 303 us a call, 9 of them the
-// merge, 4.4 TB/s of the copy's 6.6 (293 without the look for small weights; the ALU pipe is 60 % busy, so the
-// conversions and the softmax of padded rows bound it, not the loads; three CTAs a SM with two stages: the same time).
-// 8 captions of 320 tokens: 8 us a call, all latency.
+// One step of 64 sequences of up to 16384 tokens, 8 key heads of 128, e4m3 (1.34 GB): 300 us a call, 9 of them the
+// merge, 4.5 TB/s of the copy's 6.6 (290 without the look for small weights; where scores spread so far that every
+// tile has some, a step takes up to 1.5 times as long). Two CTAs, 8 warps, a SM issue 0.55 instructions a cycle and
+// scheduler, the ALU pipe is 54 % busy: conversions and the softmax of padded rows, with too few warps to cover their
+// chain, not the loads (three CTAs a SM with two stages: the same time). 8 captions of 320 tokens: 8 us a call, all
+// latency.
 #include <ATen/cuda/CUDAContext.h>
 #include <torch/extension.h>
 
@@ -320,8 +322,9 @@ __global__ void __launch_bounds__(kWarps * 32, 2) paged_rows_kernel(const PagedA
     float ms[2];
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
-      const float mq = quad_max(mt[r]), top = Q8 && mq - (mq - kTop) <= kTop ? mq - kTop : mq;  // (rounding, infinities)
-      const float mn = fmaxf(m[r], top);
+      const float mq = quad_max(mt[r]);
+      // less kTop, but where rounding or an infinity would let a weight pass 2^kTop
+      const float mn = fmaxf(m[r], Q8 && mq - (mq - kTop) <= kTop ? mq - kTop : mq);
       ms[r] = mn == -INFINITY ? 0.f : mn;  // no visible key yet: weights 2^(-inf) = 0
       const float c = ex2_ftz(m[r] - ms[r]);
       m[r] = mn;

@@ -25,8 +25,9 @@
 // 4 prompts of up to 1000 new tokens over 8192, 16 / 8 heads of 128 in bf16 (124 GFLOP): 147 us and 17 us for the
 // merge of the cut items; the products alone are 2648 cycles a tile pair (isolated), a pair takes about 3700, two
 // halves of softmax at 1500 being the longer half of the chain (the exponentials alone are 1024). The roles' code
-// competes for the instruction cache: one copy of each role's loop took captions from 150 to 97 us and e4m3 chunks
-// from 1790 to 1200. e4m3 tiles are bound by their conversion (four warps, 1.6 to 2.6 thousand cycles an operand).
+// competes for the instruction cache (tensor pipe 39 %, special functions 39 %, issue slots 34 % of the launch): one
+// copy of each role's loop took captions from 150 to 97 us and e4m3 chunks from 1790 to 1200. e4m3 tiles are bound by
+// their conversion (four warps, 1.6 to 2.6 thousand cycles an operand).
 //
 // Slots past the keys a CTA may see are zero in V's tile (whatever the pool holds there); in K's tile they are masked.
 // TMEM: S_A [0, 64) and [64, 128), S_B [128, 192) and [192, 256), O_A [256, 256 + D), O_B [256 + D, 256 + 2 D).

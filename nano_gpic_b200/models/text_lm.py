@@ -47,7 +47,8 @@ def check_model(model):
     rope = getattr(c, "rope_parameters", None) or getattr(c, "rope_scaling", None) or {}
     kind = rope.get("rope_type", rope.get("type", "default"))
     if kind not in ROPE_TYPES or getattr(model.rotary_emb, "attention_scaling", 1.0) != 1.0:
-        raise ValueError(f"TextLM: rotary embedding of type {ROPE_TYPES} without attention scaling expected, got {kind!r}")
+        raise ValueError(f"TextLM: rotary embedding of type {ROPE_TYPES} without attention scaling expected, got "
+                         f"{kind!r}")
     rest = sorted(k for k in model.state_dict() if not k.startswith("rotary_emb.") and not k.endswith(WEIGHTS))
     if rest:
         raise ValueError(f"TextLM: no use for the model's {rest}")

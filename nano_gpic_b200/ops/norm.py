@@ -153,7 +153,8 @@ def add_rms_bwd(dh, ds, s, rstd, w, dw_acc=None):
     """Gradient of add_rms_fwd: dh [M, C] bf16 (of h), ds [M, C] in s's type (of s as the later blocks read it) or None,
     s and rstd as the forward returned them. Returns dx [M, C] in s's type, the gradient of x and of res alike:
         xn = s * rstd, dxn = dh * w, dx = rstd * (dxn - xn * mean(dxn * xn)) + ds
-    dw_acc [C] fp32: sum over rows of dh * xn is added into it (fixed order: the same inputs give the same bits)."""
+    dw_acc [C] fp32: sum over rows of dh * xn is added into it (fixed order: the same inputs give the same bits). For a
+    bf16 stream this is rms_mod_bwd without modulation, dres = ds."""
     if not dh.is_cuda:
         _add_rms_check(dh, s, w)
         xn = s.float() * rstd[:, None]

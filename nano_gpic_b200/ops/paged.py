@@ -145,9 +145,10 @@ def paged_attn(q, cache, table, total, cu, max_new, max_total, scale=None, causa
 
     Sequence b has total[b] tokens in the cache (int32 [B]), its new ones last and already written: row i of its n new
     rows sees tokens 0 .. total[b] - n + i (causal), or all total[b]. A row that sees none gets o = 0, lse = -inf.
+    A NaN in a row's query, or in a key that it sees, makes its o and lse NaN.
     max_new and max_total are the host's upper bounds on the new rows and on total of any sequence: they choose the
-    launch, and a sequence beyond them sets the device status word. Rows past cu[B] hold no result. scale (positive)
-    defaults to 1 / sqrt(D).
+    launch (as far as q's rows and the table's columns go, so a loose bound is no harm), and a sequence beyond them sets
+    the device status word. Rows past cu[B] hold no result. scale (positive) defaults to 1 / sqrt(D).
     Returns (o [T, H * D] bf16, lse [T, H] fp32, natural log)."""
     D = cache.k.shape[3]
     if scale is None:

@@ -1,7 +1,8 @@
 """The extension's device error word: kernels that give up a bounded wait record a code there instead of hanging.
 
 Codes (csrc/common.cuh): 1 stage-full wait, 2 stage-empty wait, 3 accumulator-full wait, 4 accumulator-empty wait,
-5 drain on unwind, 6 peer flag, 7 page table, 8 length bound. `check()` raises NanoCommTimeout / RuntimeError when the word is set.
+5 drain on unwind, 6 peer flag, 7 page table, 8 length bound. `check()` raises NanoCommTimeout / RuntimeError when the
+word is set.
 """
 from .._ext import ext
 
