@@ -96,7 +96,7 @@ class Qwen3TextEncoder(BaseConditioner):
     directly (e.g. a randomly initialised Qwen3Model from a config, and any callable tokenizer). native="bf16" or "e4m3"
     runs the model on the framework's kernels (models/text_lm.py) with a key/value cache of that type instead of through
     transformers; its projections are a second copy of the model's, laid out at the first caption and again when the
-    module was moved or its weights were replaced."""
+    module was moved or its weights were replaced (not through .data, which torch does not count)."""
 
     def __init__(self, weight_path=None, embed_dim=None, max_length=128, pad_multiple=8, model=None, tokenizer=None,
                  device=None, native=None):

@@ -40,7 +40,10 @@ ROPE_TYPES = ("default", "linear", "llama3")
 def check_model(model):
     """Raises for what a Qwen3Model may have and the blocks above do not compute."""
     c = model.config
-    if set(c.layer_types) != {"full_attention"}:
+    # (configs without layer_types say it once for all layers)
+    kinds = getattr(c, "layer_types", None) or [
+        "sliding_attention" if getattr(c, "use_sliding_window", False) else "full_attention"]
+    if set(kinds) != {"full_attention"}:
         raise ValueError("TextLM: full attention in every layer expected, the model has a sliding window")
     if c.hidden_act not in ("silu", "swish"):
         raise ValueError(f"TextLM: hidden_act must be 'silu', got {c.hidden_act!r}")

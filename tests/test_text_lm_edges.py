@@ -130,3 +130,13 @@ def test_head_dim_128_gpu(kind, chunk, lim):
     from nano_gpic_b200.ops import status
     _at_head_dim_128("cuda", kind, chunk, lim)
     status.check()
+
+
+def test_a_config_without_layer_types():
+    from nano_gpic_b200.models.text_lm import check_model
+    m = _qwen3()
+    m.config.layer_types = None
+    check_model(m)
+    m.config.use_sliding_window = True
+    with pytest.raises(ValueError, match="sliding window"):
+        check_model(m)
